@@ -118,6 +118,41 @@ class PrepareArgs(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    """Mirror of hb_kv_cache."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("k_stride_p", C.c_int64), ("k_stride_h", C.c_int64), ("k_stride_s", C.c_int64),
+        ("v_stride_p", C.c_int64), ("v_stride_h", C.c_int64), ("v_stride_s", C.c_int64),
+        ("num_pages", C.c_int32), ("page_size", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("starts", C.c_void_p), ("table_stride", C.c_int64),
+        ("max_pages", C.c_int32), ("B", C.c_int32), ("T", C.c_int32),
+    ]
+
+
+class KvAppendArgs(C.Structure):
+    """Mirror of hb_kv_append_args."""
+    _fields_ = [
+        ("cache", KvCache), ("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+        ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64), ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
+        ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("qo_stride_t", C.c_int64), ("qo_stride_h", C.c_int64),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_len", C.c_int32), ("Hq", C.c_int32), ("dtype", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class FaPagedArgs(C.Structure):
+    """Mirror of hb_fa_paged_args."""
+    _fields_ = [
+        ("cache", KvCache), ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("o_stride_t", C.c_int64), ("o_stride_h", C.c_int64),
+        ("Hq", C.c_int32), ("max_tokens", C.c_int32), ("causal", C.c_int32), ("softmax_scale", C.c_float), ("dtype", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+CACHE_FAULTS = {1: "page", 2: "length", 4: "starts", 8: "position"}  # hb_cache_fault
+
 EW_OPS = {
     "load": 0, "add": 1, "sub": 2, "rsub": 3, "mul": 4, "div": 5, "rdiv": 6, "max": 7, "min": 8, "pow": 9,
     "neg": 16, "abs": 17, "exp": 18, "log": 19, "log2": 20, "sqrt": 21, "rsqrt": 22, "recip": 23, "sigmoid": 24,
@@ -151,6 +186,7 @@ ROWWISE_AUTO, ROWWISE_INTERPRET, ROWWISE_COMPILED = 0, 1, 2
 # every symbol include/heddle_b200.h declares
 EXPORTS = (
     "hb_fa_fwd", "hb_fa_fwd_workspace", "hb_fa_fwd_ws", "hb_fa_fwd_noalloc", "hb_status_word_noalloc", "hb_fa_bwd_preprocess", "hb_fa_bwd_dkdv", "hb_fa_bwd_dkdv_workspace", "hb_fa_bwd_dkdv_ws", "hb_fa_bwd_dq", "hb_fa_bwd", "hb_h2o_score", "hb_gemm_epilogue", "hb_rms_rowstat", "hb_prepare_weight", "hb_row_softmax", "hb_rowwise_program", "hb_rowwise_compiler_available", "hb_debug_rowwise_compile", "hb_status_word",
+    "hb_kv_append", "hb_fa_paged_workspace", "hb_fa_paged", "hb_cache_status",
     "hb_version",
     "hb_query", "hb_last_error", "hb_shutdown", "hb_debug_umma", "hb_debug_wait_timeout", "hb_debug_fa_fwd_stages",
 )
@@ -236,6 +272,14 @@ def load() -> C.CDLL:
     lib.hb_rowwise_compiler_available.restype = C.c_int
     lib.hb_debug_rowwise_compile.argtypes = [C.POINTER(RowwiseArgs), C.c_char_p, C.c_int64]
     lib.hb_debug_rowwise_compile.restype = C.c_int
+    lib.hb_kv_append.argtypes = [C.POINTER(KvAppendArgs)]
+    lib.hb_kv_append.restype = C.c_int
+    lib.hb_fa_paged_workspace.argtypes = [C.POINTER(FaPagedArgs), C.POINTER(C.c_uint64)]
+    lib.hb_fa_paged_workspace.restype = C.c_int
+    lib.hb_fa_paged.argtypes = [C.POINTER(FaPagedArgs), C.c_void_p, C.c_uint64]
+    lib.hb_fa_paged.restype = C.c_int
+    lib.hb_cache_status.argtypes = [C.POINTER(C.c_uint32)]
+    lib.hb_cache_status.restype = C.c_int
     lib.hb_status_word.argtypes = [C.POINTER(C.c_uint32)]
     lib.hb_status_word.restype = C.c_int
     lib.hb_status_word_noalloc.argtypes = [C.POINTER(C.c_uint32), C.c_void_p]

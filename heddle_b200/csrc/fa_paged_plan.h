@@ -1,0 +1,31 @@
+// How the rows kernel of the paged attention (fa_paged_sm100.cuh) shares out its work: ONE list of key tiles over all (sequence, KV head,
+// row tile) items, cut into equal runs.  The lengths are known on the device only, so every block works its run out from them.
+// Shared by the kernels and a test on the CPU.
+#pragma once
+
+#include <stdint.h>
+
+#include "fast_div.h"
+
+namespace hb {
+
+constexpr int kPagedTile = 32;   // keys of a tile: what a warp works through at a time
+constexpr int kPagedWarps = 4;   // of a block; they take the tiles of its run in turn
+
+// Key tiles of an item with `len` keys (an item without keys has a tile all the same: somebody has to write its rows).
+HB_HD int paged_tiles(int len) { return len <= 0 ? 1 : (len + kPagedTile - 1) / kPagedTile; }
+HB_HD int paged_row_tiles(int n, int group, int rows) {
+  return static_cast<int>((static_cast<long long>(n) * group + rows - 1) / rows);
+}
+// Of `blocks` blocks those that get a run: no run is shorter than a tile for every warp.
+HB_HD int paged_runs(long long total, int blocks) {
+  const long long most = (total + kPagedWarps - 1) / kPagedWarps;
+  return static_cast<int>(most < blocks ? (most < 1 ? 1 : most) : blocks);
+}
+HB_HD long long paged_begin(long long total, int runs, int w) {  // total < 2^48, runs < 2^12
+  return total / runs * w + total % runs * w / runs;
+}
+// The run of tile t: the last w with begin(w) = floor(w total / runs) <= t.
+HB_HD int paged_run_of(long long total, int runs, long long t) { return static_cast<int>(((t + 1) * runs - 1) / total); }
+
+}  // namespace hb

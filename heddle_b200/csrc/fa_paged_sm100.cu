@@ -1,0 +1,131 @@
+// hb_fa_paged: checks, the workspace and the launches of the paged attention (fa_paged_sm100.cuh).
+#include "fa_paged_sm100.cuh"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <mutex>
+
+#include "host_common.h"
+
+namespace hb {
+
+static std::mutex g_paged_mutex;
+
+static int paged_check(const char* fn, const hb_fa_paged_args* a, bool* empty) {
+  if (a == nullptr) return set_error(HB_ERR_BAD_ARG, "%s: args is NULL", fn);
+  const hb_kv_cache& c = a->cache;
+  const int rc = kv_cache_check(fn, c, empty);
+  if (rc != HB_OK) return rc;
+  if (a->dtype != HB_BF16 && a->dtype != HB_FP16) return set_error(HB_ERR_UNSUPPORTED, "%s: dtype %d (bf16 and fp16 are built)", fn, a->dtype);
+  if (a->Hq <= 0 || a->Hq % c.Hkv != 0) return set_error(HB_ERR_BAD_ARG, "%s: Hq = %d must be a multiple of Hkv = %d", fn, a->Hq, c.Hkv);
+  if (static_cast<int64_t>(c.T) * a->Hq > 0x7fffffffll || static_cast<int64_t>(c.B) * a->Hq > 0x7fffffffll)
+    return set_error(HB_ERR_UNSUPPORTED, "%s: T * Hq and B * Hq may not exceed 2^31", fn);
+  if (*empty) return HB_OK;
+  if (a->q == nullptr || a->o == nullptr) return set_error(HB_ERR_BAD_ARG, "%s: NULL pointer", fn);
+  const uint64_t bits = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->o) |
+                        static_cast<uint64_t>(2 * (a->q_stride_t | a->q_stride_h | a->o_stride_t | a->o_stride_h));
+  if ((bits & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0)
+    return set_error(HB_ERR_ALIGN, "%s: rows of q and o must be 16-byte aligned, lse 4-byte aligned", fn);
+  return HB_OK;
+}
+
+// Query rows of a (sequence, KV head) at most, INT_MAX where the call does not say.
+static int64_t paged_most_rows(const hb_fa_paged_args* a) {
+  const hb_kv_cache& c = a->cache;
+  const int64_t group = a->Hq / c.Hkv;
+  if (c.starts == nullptr) return group * (c.T / c.B);
+  return a->max_tokens > 0 ? group * std::min(a->max_tokens, c.T) : INT_MAX;
+}
+static int paged_tile_rows(const hb_fa_paged_args* a) { return paged_most_rows(a) <= 8 ? 8 : kPagedMaxRows; }
+
+static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
+  const uint64_t blocks = 2ull * sm_count, rows = paged_tile_rows(a);
+  return 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
+}
+
+template <typename T, int D, int kRows>
+static int launch_rows(const FaPagedParams& p, int blocks, cudaStream_t stream) {
+  using Smem = FaPagedSmem<D, kRows>;
+  auto kernel = fa_paged_rows_kernel<T, D, kRows>;
+  static bool configured[64] = {};
+  int dev = 0;
+  HB_CUDA_CHECK(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(g_paged_mutex);
+    if (!configured[dev & 63]) {
+      HB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)));
+      configured[dev & 63] = true;
+    }
+  }
+  HB_CUDA_CHECK(launch_dependent(kernel, blocks, kPagedThreads, sizeof(Smem), stream, 0, p));
+  // an item of few has parts in many runs: a warp of the merge for every four
+  const long long items = static_cast<long long>(p.c.B) * p.c.Hkv;
+  const long long parts = (blocks + items - 1) / items + 1;
+  const unsigned warps = static_cast<unsigned>(std::min<long long>(kPagedCombineWarps, (parts + 3) / 4));
+  HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D>, blocks * kRows, 32 * warps, 0, stream, 0, p, kRows));
+  return HB_OK;
+}
+template <typename T>
+static int launch_rows_of(const FaPagedParams& p, int D, int rows, int blocks, cudaStream_t stream) {
+  if (D == 128) return rows == 8 ? launch_rows<T, 128, 8>(p, blocks, stream) : launch_rows<T, 128, 16>(p, blocks, stream);
+  return rows == 8 ? launch_rows<T, 64, 8>(p, blocks, stream) : launch_rows<T, 64, 16>(p, blocks, stream);
+}
+
+}  // namespace hb
+
+extern "C" int hb_fa_paged_workspace(const hb_fa_paged_args* a, uint64_t* bytes) {
+  using namespace hb;
+  clear_error();
+  if (bytes == nullptr) return set_error(HB_ERR_BAD_ARG, "hb_fa_paged_workspace: bytes is NULL");
+  *bytes = 0;
+  bool empty = false;
+  int rc = paged_check("hb_fa_paged_workspace", a, &empty);
+  if (rc != HB_OK || empty) return rc;
+  DeviceState* st = nullptr;
+  rc = get_device_state(&st);
+  if (rc != HB_OK) return rc;
+  *bytes = paged_workspace(a, st->sm_count);
+  return HB_OK;
+}
+
+extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t bytes) {
+  using namespace hb;
+  clear_error();
+  bool empty = false;
+  int rc = paged_check("hb_fa_paged", a, &empty);
+  if (rc != HB_OK || empty) return rc;
+  DeviceState* st = nullptr;
+  rc = get_device_state(&st);
+  if (rc != HB_OK) return rc;
+  const uint64_t need = paged_workspace(a, st->sm_count);
+  if (workspace == nullptr || bytes < need)
+    return set_error(HB_ERR_BAD_ARG, "hb_fa_paged: needs a workspace of %llu bytes, got %llu", (unsigned long long)need,
+                     (unsigned long long)(workspace == nullptr ? 0 : bytes));
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return set_error(HB_ERR_ALIGN, "hb_fa_paged: the workspace must be 16-byte aligned");
+  const hb_kv_cache& c = a->cache;
+  const int rows = paged_tile_rows(a), blocks = 2 * st->sm_count;
+  FaPagedParams p;
+  p.c = kv_view(c, st);
+  p.q = a->q;
+  p.o = a->o;
+  p.lse = a->lse;
+  p.q_st = a->q_stride_t;
+  p.q_sh = a->q_stride_h;
+  p.o_st = a->o_stride_t;
+  p.o_sh = a->o_stride_h;
+  p.Hq = a->Hq;
+  p.group = a->Hq / c.Hkv;
+  p.causal = a->causal ? 1 : 0;
+  p.row_limit = INT_MAX;
+  p.by_group = make_fast_div(p.group);
+  const float scale = a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c.D);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.heads = static_cast<PagedHead*>(workspace);
+  p.part_o = reinterpret_cast<float*>(p.heads + blocks);
+  p.part_lse = p.part_o + 2ll * blocks * rows * c.D;
+  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+  return a->dtype == HB_BF16 ? launch_rows_of<__nv_bfloat16>(p, c.D, rows, blocks, stream)
+                             : launch_rows_of<__half>(p, c.D, rows, blocks, stream);
+}

@@ -71,8 +71,9 @@ int get_device_state(DeviceState** out) {
                        "device %d has compute capability %d.%d; this library is built for sm_100a only", dev, major,
                        minor);
     }
-    HB_CUDA_CHECK(cudaMalloc(&st.status_word, sizeof(uint32_t)));
-    HB_CUDA_CHECK(cudaMemset(st.status_word, 0, sizeof(uint32_t)));
+    HB_CUDA_CHECK(cudaMalloc(&st.status_word, 2 * sizeof(uint32_t)));
+    HB_CUDA_CHECK(cudaMemset(st.status_word, 0, 2 * sizeof(uint32_t)));
+    st.cache_fault = st.status_word + 1;
     st.device = dev;
   }
   if (g_encode == nullptr) {
@@ -158,6 +159,23 @@ int hb_status_word(uint32_t* out) {
   HB_CUDA_CHECK(cudaMemcpy(out, st->status_word, sizeof(uint32_t), cudaMemcpyDeviceToHost));
   if (*out != 0) return hb::set_error(HB_ERR_TIMEOUT, "hb_status_word: %s", hb::describe_status(*out));
   return HB_OK;
+}
+
+int hb_cache_status(uint32_t* out) {
+  hb::clear_error();
+  if (out == nullptr) return hb::set_error(HB_ERR_BAD_ARG, "hb_cache_status: out is NULL");
+  hb::DeviceState* st = nullptr;
+  int rc = hb::get_device_state(&st);
+  if (rc != HB_OK) return rc;
+  HB_CUDA_CHECK(cudaDeviceSynchronize());
+  HB_CUDA_CHECK(cudaMemcpy(out, st->cache_fault, sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  if (*out == 0) return HB_OK;
+  HB_CUDA_CHECK(cudaMemset(st->cache_fault, 0, sizeof(uint32_t)));
+  return hb::set_error(HB_ERR_BAD_ARG, "hb_cache_status: 0x%x:%s%s%s%s", *out,
+                       *out & HB_CACHE_BAD_PAGE ? " a page outside of the cache;" : "",
+                       *out & HB_CACHE_BAD_LENGTH ? " a length that does not fit its page table row or its tokens;" : "",
+                       *out & HB_CACHE_BAD_STARTS ? " starts that descend or leave the tokens;" : "",
+                       *out & HB_CACHE_BAD_POSITION ? " a position behind the rotary tables;" : "");
 }
 
 int hb_shutdown(void) {

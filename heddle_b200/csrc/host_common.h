@@ -32,6 +32,7 @@ struct DeviceState {
   int smem_optin = 0;
   int cc = 0;
   uint32_t* status_word = nullptr;  // device memory, zero-initialised
+  uint32_t* cache_fault = nullptr;  // the word behind it: what the cache kernels found wrong (hb_cache_fault bits)
 };
 
 // Lazily created state of the CURRENT device (mutex-guarded).  Returns an hb_status.

@@ -10,7 +10,7 @@ import functools
 import math
 import os
 import struct
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -673,3 +673,166 @@ def h2o_score(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, causal: bo
         _stream_ptr(q.device))
     _call(q.device, _lib.load().hb_h2o_score, C.byref(a))
     return score
+
+
+class KvPages(NamedTuple):
+    """Pages of a key/value cache: e4m3 codes and a power-of-two fp32 scale for each (page, head).  ``layout`` "bhsd": ``k`` and ``v``
+    are [num_pages, Hkv, page_size, D]; "bshd": [num_pages, page_size, Hkv, D]; any strides, head_dim contiguous.  The scales are
+    [num_pages, Hkv].  Token t of sequence b is in page ``page_table[b, t // page_size]``, at place ``t % page_size``."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    layout: str = "bhsd"
+
+
+def kv_pages(num_pages: int, page_size: int, kv_heads: int, head_dim: int, *, layout: str = "bhsd", device=None) -> KvPages:
+    """Empty pages for ``kv_append`` and ``fa_paged``: page_size 16, 32, 64 or 128, head_dim 64 or 128."""
+    if page_size not in (16, 32, 64, 128) or head_dim not in (64, 128) or num_pages < 0 or kv_heads < 1:
+        raise ValueError("kv_pages: page_size is 16, 32, 64 or 128, head_dim 64 or 128, kv_heads at least 1")
+    if layout not in ("bhsd", "bshd"):
+        raise ValueError(f"unknown layout {layout!r}")
+    shape = (num_pages, kv_heads, page_size, head_dim) if layout == "bhsd" else (num_pages, page_size, kv_heads, head_dim)
+    device = "cuda" if device is None else device
+    codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
+    return KvPages(*codes, *scales, layout)
+
+
+def _kv_cache(who: str, pages: KvPages, page_table, seq_lens, starts, x) -> "_lib.KvCache":
+    """``hb_kv_cache`` for rows ``x`` [T, heads, D] of a call; everything the host can see is checked."""
+    k, v, k_scale, v_scale, layout = pages
+    device = x.device
+    for t in (k, v, k_scale, v_scale, page_table, seq_lens, starts):
+        if t is not None and t.device != device:
+            _require_cuda(t)
+            raise ValueError(f"{who}: all tensors must be on {device}, got one on {t.device}")
+    if layout == "bhsd":
+        h_ax, s_ax = 1, 2
+    elif layout == "bshd":
+        h_ax, s_ax = 2, 1
+    else:
+        raise ValueError(f"unknown layout {layout!r}")
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
+        raise ValueError(f"{who}: pages of keys and values must be 4-D and alike, got {tuple(shape)} and {tuple(v.shape)}")
+    ks, vs = k.stride(), v.stride()
+    if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn:
+        raise TypeError(f"{who}: pages hold torch.float8_e4m3fn, got {k.dtype} and {v.dtype}")
+    num_pages, heads, D = shape[0], shape[h_ax], shape[3]
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError(f"{who}: the last axis of the pages must be contiguous")
+    for t in (k_scale, v_scale):
+        if t.dtype is not torch.float32 or t.shape != (num_pages, heads) or not t.is_contiguous():
+            raise ValueError(f"{who}: scales must be contiguous fp32 [num_pages, Hkv] = {(num_pages, heads)}")
+    if x.dim() != 3 or x.shape[2] != D:
+        raise ValueError(f"{who}: rows must be [tokens, heads, {D}], got {tuple(x.shape)}")
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"{who}: page_table must be int32 [sequences, max_pages] with a contiguous last axis")
+    B, max_pages = page_table.shape
+    if seq_lens.dtype is not torch.int32 or seq_lens.shape != (B,) or not seq_lens.is_contiguous():
+        raise ValueError(f"{who}: seq_lens must be contiguous int32 [{B}]")
+    if starts is not None and (starts.dtype is not torch.int32 or starts.shape != (B + 1,) or not starts.is_contiguous()):
+        raise ValueError(f"{who}: starts must be contiguous int32 [{B + 1}]")
+    return _lib.KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ks[0], ks[h_ax], ks[s_ax], vs[0], vs[h_ax], vs[s_ax],
+                        num_pages, shape[s_ax], heads, D, page_table.data_ptr(), seq_lens.data_ptr(),
+                        starts.data_ptr() if starts is not None else None, page_table.stride(0), max_pages, B, x.shape[0])
+
+
+def _rows_16(t: torch.Tensor) -> torch.Tensor:
+    """[tokens, heads, D] whose rows the library can read: head_dim contiguous, every row 16-byte aligned."""
+    s = t.stride()
+    return t if s[2] == 1 and not (s[0] | s[1]) % 8 and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, pages: KvPages, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
+              starts: Optional[torch.Tensor] = None, rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+              q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write the keys and values of new tokens into ``pages`` through ``hb_kv_append``, the keys rotated by their positions.
+
+    ``k``, ``v`` [T, Hkv, D] bf16 or fp16 (any token and head strides: views of a merged projection are read in place) are the last
+    tokens of ``page_table.shape[0]`` sequences: rows ``starts[b]`` to ``starts[b + 1]`` (int32, None: as many for each) belong to
+    sequence b, and ``seq_lens`` (int32) counts them.  ``page_table`` int32 [sequences, max_pages].  The three are read on the
+    device, so a captured call takes what they hold at its replay; what is wrong in them is left out and reported by
+    ``cache_status``.  ``rope`` = (cos, sin), fp32 [positions, D / 2], rotate-half as in ``gemm_epilogue``.  ``q`` [T, Hq, D]: the
+    queries of the same tokens; they are returned rotated (rows of no sequence hold anything), as a new tensor.
+
+    A page whose first place is written starts anew; in a page that holds earlier tokens of its sequence the scale grows where the
+    new ones need it, and the earlier codes are rounded to it.  A token with an infinity or NaN in a head's key or value becomes a
+    NaN key and a zero value there.  Two sequences may share pages that neither appends to."""
+    _require_cuda(k, v, q)
+    if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise TypeError(f"kv_append takes bf16 or fp16 rows of one dtype, got {k.dtype}, {v.dtype}" + (f", {q.dtype}" if q is not None else ""))
+    cache = _kv_cache("kv_append", pages, page_table, seq_lens, starts, k)
+    if k.shape[1] != cache.Hkv or v.shape != k.shape:
+        raise ValueError(f"kv_append: k and v must be [tokens, {cache.Hkv}, {cache.D}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    device = k.device
+    if v.device != device or (q is not None and q.device != device):
+        raise ValueError("kv_append: all tensors must be on one device")
+    k, v = _rows_16(k), _rows_16(v)
+    ks, vs = k.stride(), v.stride()
+    a = _lib.KvAppendArgs(cache, k.data_ptr(), v.data_ptr(), None, None, ks[0], ks[1], vs[0], vs[1])
+    out = None
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != cache.D or q.shape[1] < 1:
+            raise ValueError(f"kv_append: q must be [{k.shape[0]}, heads, {cache.D}], got {tuple(q.shape)}")
+        q = _rows_16(q)
+        out = q.new_empty(q.shape)
+        qs = q.stride()
+        a.q, a.q_out, a.Hq = q.data_ptr(), out.data_ptr(), q.shape[1]
+        a.q_stride_t, a.q_stride_h, a.qo_stride_t, a.qo_stride_h = qs[0], qs[1], q.shape[1] * cache.D, cache.D
+    if rope is not None:
+        cos, sin = (_as_fp32(t) for t in rope)
+        _require_cuda(cos, sin)
+        if cos.dim() != 2 or cos.shape[1] * 2 != cache.D or sin.shape != cos.shape or cos.device != device or sin.device != device:
+            raise ValueError(f"kv_append: rope tables must be [positions, {cache.D // 2}] on {device}")
+        if (cos.data_ptr() | sin.data_ptr()) % 16:
+            cos, sin = cos.clone(), sin.clone()
+        a.rope_cos, a.rope_sin, a.rope_len = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    a.dtype, a.stream = _DTYPES[k.dtype], _stream_ptr(device)
+    _call(device, _lib.load().hb_kv_append, C.byref(a))
+    return out
+
+
+def fa_paged(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
+             starts: Optional[torch.Tensor] = None, max_tokens: Optional[int] = None, causal: bool = True,
+             softmax_scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+             ) -> "torch.Tensor | Tuple[torch.Tensor, torch.Tensor]":
+    """Attention over a paged 8-bit cache through ``hb_fa_paged``: one token a sequence, a few, prompts, or a batch of all.
+
+    ``q`` [T, Hq, D] bf16 or fp16 are the last tokens of each sequence, ``starts``, ``seq_lens`` and ``page_table`` as in
+    ``kv_append`` (which comes first: ``seq_lens`` counts the queries' own tokens).  A query sees its sequence's keys, with ``causal``
+    those up to its own position.  ``max_tokens``: the most rows a sequence has, where ``starts`` is given (a hint that chooses
+    kernels).  Returns O [T, Hq, D] in q's dtype and, if requested, the natural-log LSE fp32 [T, Hq]; rows without a
+    visible key are 0 and -inf.  Rows of no sequence are left as they are in ``out`` (and are whatever new memory holds otherwise)."""
+    _require_cuda(q, out)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"fa_paged takes bf16 or fp16 queries, got {q.dtype}")
+    cache = _kv_cache("fa_paged", pages, page_table, seq_lens, starts, q)
+    device = q.device
+    q = _rows_16(q)
+    T, Hq, D = q.shape
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != device:
+        raise ValueError("out must match q's shape, dtype and device and have a contiguous last axis")
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
+    qs, os_ = q.stride(), out.stride()
+    a = _lib.FaPagedArgs(cache, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, qs[0], qs[1], os_[0], os_[1],
+                         Hq, int(max_tokens) if max_tokens is not None else 0, 1 if causal else 0,
+                         float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D), _DTYPES[q.dtype], _stream_ptr(device))
+    lib, arg, need = _lib.load(), C.byref(a), C.c_uint64(0)
+    _call(device, lib.hb_fa_paged_workspace, arg, C.byref(need))
+    ws = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    _call(device, lib.hb_fa_paged, arg, ws.data_ptr() if ws is not None else None, need.value)
+    return (out, lse) if return_lse else out
+
+
+def cache_status() -> int:
+    """What ``kv_append`` and ``fa_paged`` found wrong in page tables, lengths and starts on the current device since the last call of
+    this function: 0, or the bits of ``_lib.CACHE_FAULTS``.  Synchronises the device and clears the word."""
+    w = C.c_uint32(0)
+    rc = _lib.load().hb_cache_status(C.byref(w))
+    if rc and not w.value:
+        _lib.check(rc)
+    return int(w.value)

@@ -454,6 +454,103 @@ int hb_rowwise_compiler_available(void);
  * `args` is dereferenced).  `source` (may be NULL) receives the generated text. */
 int hb_debug_rowwise_compile(const hb_rowwise_args* args, char* source, int64_t capacity);
 
+/*
+ * The paged key/value cache: pages of page_size tokens, keys and values as e4m3 codes with one fp32 scale for each (page, head),
+ * a power of two, so that a value is code * scale exactly.  No counterpart in the reference, which has no cache.
+ *   k, v              codes [num_pages, Hkv, page_size, D] by strides (in codes; D contiguous, rows 16-byte aligned)
+ *   k_scale, v_scale  [num_pages, Hkv] fp32 contiguous
+ *   page_table        int32 [B, max_pages], row stride table_stride: token t of sequence b is in page page_table[b][t / page_size], at
+ *                     place t % page_size
+ *   seq_lens          int32 [B]: tokens of each sequence, those of the call included
+ *   starts            int32 [B + 1], ascending: the rows [starts[b], starts[b + 1]) of the call's k, v, q and outputs are the last tokens of
+ *                     sequence b.  NULL: T / B rows for every sequence.  Rows outside of all sequences are neither read nor written.
+ * page_table, seq_lens and starts are read on the device: a captured call takes what they hold when it is replayed.  Entries of the
+ * page table behind a sequence's last page are not read.  What the device finds wrong in them it leaves out and reports
+ * through hb_cache_status: a page outside of [0, num_pages) (its tokens are not written, and are not seen by any query), a
+ * length beyond max_pages * page_size (taken as that), more rows than the sequence is long, a position behind the rotary tables
+ * (neither written), starts that descend or leave [0, T] (taken as the nearest that do not).
+ * page_size 16, 32, 64 or 128; D 64 or 128.
+ */
+typedef struct hb_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_stride_p, k_stride_h, k_stride_s; /* page, head, token */
+  int64_t v_stride_p, v_stride_h, v_stride_s;
+  int32_t num_pages, page_size, Hkv, D;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* starts;
+  int64_t table_stride;
+  int32_t max_pages, B, T;
+} hb_kv_cache;
+
+/*
+ * Append: the call's keys, rotated by their positions, and values are written into the pages as codes.  A page whose first token is
+ * among them starts anew: what it held does not count.  Its scale is the smallest power of two (2^-100 to 2^119) that takes the
+ * largest magnitude to at most 448; in a page that holds earlier tokens of the sequence the scale grows where the new ones
+ * need it, and the earlier codes are then rounded again to the new scale.  A token whose key or value holds an infinity or
+ * a NaN (or whose key does once rotated) becomes a NaN key and a zero value in that head: a query that sees it is NaN, no other.
+ * A page takes tokens of one sequence in a call; no other work may use its pages meanwhile.
+ *   k, v   [T, Hkv, D]; q (may be NULL) [T, Hq, D], rotated into q_out [T, Hq, D] (may be q itself); 16-bit, by strides
+ *   rope_cos, rope_sin  fp32 [rope_len, D / 2] contiguous, indexed by position; both NULL: nothing is rotated
+ * Rotation pairs i with i + D/2: x_i cos - x_{i+D/2} sin and x_{i+D/2} cos + x_i sin, products and sums rounded to fp32 each.
+ */
+typedef struct hb_kv_append_args {
+  hb_kv_cache cache;
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h;
+  const float* rope_cos;
+  const float* rope_sin;
+  int32_t rope_len, Hq;
+  int32_t dtype; /* HB_BF16 or HB_FP16 */
+  void* stream;
+} hb_kv_append_args;
+
+int hb_kv_append(const hb_kv_append_args* args);
+
+/*
+ * Attention of the call's queries over the cache:  O = softmax(Q K^T * softmax_scale + mask) V, optionally the natural-log LSE.
+ * A query at position p sees the keys [0, seq_lens[b]), with `causal` those at positions up to p.  Rows without a visible
+ * key are 0 with an LSE of -inf.  Query head h reads KV head h / (Hq / Hkv).
+ * Queries enter the product to 8 (bf16: all of them) or 11 (fp16: all) significant bits, no finer than 2^-17 of their row's largest;
+ * P is rounded to 8 significant bits, sums are fp32.  Which SM has which keys follows from seq_lens and starts and from the
+ * device's SMs: results repeat for equal ones, and agree within rounding between batches.
+ * A NaN code among the values of a page may reach every query whose tile of keys holds it: hb_kv_append writes none.
+ *   max_tokens  the most rows of a sequence (a hint: it chooses kernels, any value gives the result); <= 0: unknown
+ * The workspace is the caller's: hb_fa_paged_workspace writes the bytes a call needs; 16-byte aligned, need not be initialised,
+ * reusable once the call's work on `stream` is done.
+ */
+typedef struct hb_fa_paged_args {
+  hb_kv_cache cache;
+  const void* q; /* [T, Hq, D] */
+  void* o;       /* [T, Hq, D] */
+  float* lse;    /* optional [T, Hq] fp32 contiguous */
+  int64_t q_stride_t, q_stride_h, o_stride_t, o_stride_h;
+  int32_t Hq, max_tokens, causal;
+  float softmax_scale; /* <= 0 selects D^-1/2 */
+  int32_t dtype;       /* HB_BF16 or HB_FP16 */
+  void* stream;
+} hb_fa_paged_args;
+
+int hb_fa_paged_workspace(const hb_fa_paged_args* args, uint64_t* bytes);
+int hb_fa_paged(const hb_fa_paged_args* args, void* workspace, uint64_t bytes);
+
+/* What the cache kernels of the current device found wrong in page tables, lengths and starts since the last call of this
+ * function (the bits of hb_cache_fault; 0: nothing).  Synchronises the device and clears the word; HB_ERR_BAD_ARG if it was not 0. */
+typedef enum hb_cache_fault {
+  HB_CACHE_BAD_PAGE = 1,     /* a page outside of [0, num_pages) */
+  HB_CACHE_BAD_LENGTH = 2,   /* a sequence longer than its page table row, or shorter than its rows of the call */
+  HB_CACHE_BAD_STARTS = 4,   /* starts that descend or leave [0, T] */
+  HB_CACHE_BAD_POSITION = 8  /* a position behind the rotary tables */
+} hb_cache_fault;
+
+int hb_cache_status(uint32_t* out);
+
 /* Device-side status word of the current device (0 = no bounded wait ever gave up);
  * reading it synchronises the device.  *out always receives the word; the return value is
  * HB_OK when it is zero and HB_ERR_TIMEOUT otherwise (hb_last_error() then names the kernel
