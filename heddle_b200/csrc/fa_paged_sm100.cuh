@@ -2,18 +2,18 @@
 //
 //   s_ij = scale (q_i . K_j) kscale[page(j)],   o_i = sum_j softmax(s_i)_j V_j vscale[page(j)],   K, V e4m3 codes
 //
-// What bounds it is reading the codes once: 2 D bytes a token and KV head, 11 cycles of an SM's share of HBM at D = 128.  Turning the
-// codes over into 16 bits alone would take half of its issue slots, so they go into the tensor cores as they are, and the
-// 16-bit operands come to them: a bf16 number has 8 significant bits, an e4m3 one 4, so q (scaled by a power of two that takes
-// its row's largest element near 448) is the sum of two e4m3 numbers exactly, three in fp16; P (times 256) is the sum of two to 8 bits.
-// mma.sync m16n8k32 on e4m3 adds in full fp32 here (sums of 2^14 and 2^-9 come out exact) and takes 1.07 cycles of an SM, four times
-// the multiplications that the 16-bit form does.  With up to 8 rows (kRows) the 16 rows of A are the first parts over the second,
-// with up to 16 every part is a product of its own.
+// What bounds it is reading the codes once: 2 D bytes a token and KV head, 11 cycles of an SM's share of HBM at D = 128.
+// The products are mma.sync m16n8k16 in fp16, which holds every code exactly, and a query too once its row is scaled by a power of two
+// (2^-39 of the row's largest element is its last place).  Codes are converted as they come from shared memory, two at an
+// instruction; 8-bit products of mma.sync are no way around that: on sm_100 they are converted as well, operand by operand and
+// product by product (5.9 cycles of an SM for m16n8k32 against 2.0 for the fp16 product of half that depth).  So the codes are A and the
+// few query rows B: S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T, and nothing is padded beyond 8 rows.
 //
 // A warp works through tiles of 32 keys alone, from its own ring in shared memory, filled by 16-byte asynchronous copies, which
-// leave out (as zeros) what lies behind the sequence.  Tokens are numbered within a group of eight so that the score that a lane
-// holds is the P that it needs, and both readings of a tile (keys along their rows, values across them) are free of
-// bank conflicts.  The four byte columns that a lane has of four value rows are turned over in registers by eight byte permutations.
+// leave out (as zeros) what lies behind the sequence.  Keys are numbered within a group of eight so that both readings of a tile (keys
+// along their rows, values across them) are free of bank conflicts; P goes from S^T's layout into B's by a transposing move,
+// and the pairs of value rows that a lane needs are put together by byte permutations.
+// A row's maximum is adopted when it grew by more than 2^7, as in fa_fwd: P' = 256 P vscale / v_ref stays within fp16.
 //
 // Work: the list of fa_paged_plan.h.  A run may start or end inside an item: such a segment leaves fp32 partial results in the
 // workspace, and fa_paged_combine_kernel merges them.
@@ -57,42 +57,45 @@ struct FaPagedSmem {
   alignas(128) uint8_t ring[kPagedWarps][kStages][2 * kTileBytes];
   float o[kPagedWarps][kRows][D];
   float ml[kPagedWarps][2][kRows];
-  float scales[kPagedWarps][kStages][4];  // keys, values of the tile's two halves; 0: a page that the cache does not have
+  alignas(16) float scales[kPagedWarps][kStages][4];  // keys, values of the tile's two halves; 0: a page that the cache does not have
   long long sums[kPagedWarps];
   long long found_at;
   int found;
 };
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two numbers rounded to e4m3 (lo in the lower byte) and what is left of them.
-__device__ __forceinline__ uint32_t e4m3_part(float& lo, float& hi) {
-  uint16_t c;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  lo -= f.x;
-  hi -= f.y;
-  return c;
+// The codes of a word's lower and upper half as fp16 pairs.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
-__device__ __forceinline__ uint32_t e4m3_last(float lo, float hi) {
-  uint16_t c;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
-  return c;
+// An 8 x 8 matrix of 16-bit numbers, a row's pair in each lane, transposed.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
-__device__ __forceinline__ uint32_t e4m3_part4(float (&x)[4]) {
-  const uint32_t a = e4m3_part(x[0], x[1]);
-  return a | (e4m3_part(x[2], x[3]) << 16);
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr) : "memory");
+  return w;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 w;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(addr) : "memory");
+  return w;
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// zeros where there is nothing to copy
+template <int kBytes>
+__device__ __forceinline__ void cp_async_if(uint32_t dst, const void* src, bool real) {
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -133,12 +136,10 @@ __device__ __forceinline__ void paged_next_item(const FaPagedParams& p, PagedCur
 template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const __grid_constant__ FaPagedParams p) {
   using Smem = FaPagedSmem<D, kRows>;
-  constexpr bool kStacked = kRows == 8;              // A holds first parts over second parts
-  constexpr bool kHalf = Pack2<T>::kFormat == 0;     // fp16: q is a sum of three
-  constexpr float kLow = kStacked ? 16.f : 1.f;      // second parts are kept times this
-  constexpr int kSteps = D / 32;                     // products along head_dim
-  constexpr int kCols = D / 8;                       // accumulator tiles of O
-  constexpr int kHalves = kRows / 8;                 // rows of a lane
+  constexpr int kSteps = D / 16;  // products along head_dim
+  constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
+  constexpr int kN = kRows / 8;   // tiles of query rows
+  constexpr float kGrowth = 7.f, kPUnit = 256.f;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -227,30 +228,54 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
     pages(page0, page1);
   }
   uint32_t ld_stage = 0;
+  // the lane's place in a copy: chunk of a row, row of a group
+  constexpr int kChunks = D / 16;
+  constexpr int kRowsAtOnce = 32 / kChunks;
+  constexpr int kCopies = 16 / kRowsAtOnce;  // of half a tile
+  const int ld_row = lane / kChunks;
+  uint32_t ld_dst[2];  // the swizzle of a row repeats every 8 rows (two copies at D = 128)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = i * kRowsAtOnce + ld_row, chunk = lane % kChunks;
+    ld_dst[i] = row * D + (D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) * 16;
+  }
+  const uint8_t* const ld_k = kv.k + ld_row * kv.k_ss + lane % kChunks * 16;
+  const uint8_t* const ld_v = kv.v + ld_row * kv.v_ss + lane % kChunks * 16;
+  const long long k_step = kRowsAtOnce * kv.k_ss, v_step = kRowsAtOnce * kv.v_ss;
   auto load = [&]() {  // one tile, or nothing behind the run's end: a group of copies either way
     if (ld_left > 0) {
       const int tok = ld.j * kPagedTile;
       const uint32_t base = smem_u32(sm.ring[warp][ld_stage]);
-      constexpr int kChunks = D / 16;          // of a row
-      constexpr int kRowsAtOnce = 32 / kChunks;
-      const int chunk = lane % kChunks;
+      const int at = tok & ((1 << kv.page_shift) - 1);  // place of the tile's first key in its page
+      const bool full = tok + kPagedTile <= ld.s.len && page0 >= 0 && page1 >= 0;
 #pragma unroll
-      for (int i = 0; i < kPagedTile / kRowsAtOnce; ++i) {
-        const int row = i * kRowsAtOnce + lane / kChunks;
-        const int page = row < 16 ? page0 : page1;
-        const bool real = page >= 0 && tok + row < ld.s.len;
-        const int place = (tok + row) & ((1 << kv.page_shift) - 1);
-        const int sw = D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
-        const uint8_t* ks = real ? kv.k + page * kv.k_sp + ld.h * kv.k_sh + place * kv.k_ss + chunk * 16 : kv.k;
-        const uint8_t* vs = real ? kv.v + page * kv.v_sp + ld.h * kv.v_sh + place * kv.v_ss + chunk * 16 : kv.v;
-        cp_async16(base + row * D + sw * 16, ks, real);
-        cp_async16(base + Smem::kTileBytes + row * D + sw * 16, vs, real);
+      for (int half = 0; half < 2; ++half) {
+        const int page = half == 0 ? page0 : page1;
+        const int place = half == 0 ? at : (kv.page_shift == 4 ? 0 : at + 16);
+        const uint8_t* ks = ld_k + page * kv.k_sp + ld.h * kv.k_sh + place * kv.k_ss;
+        const uint8_t* vs = ld_v + page * kv.v_sp + ld.h * kv.v_sh + place * kv.v_ss;
+        if (full) {
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i, ks += k_step, vs += v_step) {
+            const uint32_t dst = base + half * 16 * D + ld_dst[i & 1] + (i >> 1) * 2 * kRowsAtOnce * D;
+            cp_async16(dst, ks);
+            cp_async16(dst + Smem::kTileBytes, vs);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i, ks += k_step, vs += v_step) {
+            const uint32_t dst = base + half * 16 * D + ld_dst[i & 1] + (i >> 1) * 2 * kRowsAtOnce * D;
+            const bool real = page >= 0 && tok + half * 16 + i * kRowsAtOnce + ld_row < ld.s.len;
+            cp_async_if<16>(dst, real ? ks : kv.k, real);
+            cp_async_if<16>(dst + Smem::kTileBytes, real ? vs : kv.v, real);
+          }
+          if (lane == 0 && ((page0 < 0 && tok < ld.s.len) || (page1 < 0 && tok + 16 < ld.s.len))) kv_report(kv, HB_CACHE_BAD_PAGE);
+        }
       }
       if (lane < 4) {
         const int page = lane & 1 ? page1 : page0;
         const float* src = (lane & 2 ? kv.v_scale : kv.k_scale) + (page >= 0 ? static_cast<long long>(page) * kv.Hkv + ld.h : 0);
-        cp_async4(smem_u32(&sm.scales[warp][ld_stage][lane]), src, page >= 0);
-        if (page < 0 && tok + 16 * (lane & 1) < ld.s.len) kv_report(kv, HB_CACHE_BAD_PAGE);
+        cp_async_if<4>(smem_u32(&sm.scales[warp][ld_stage][lane]), src, page >= 0);
       }
       if (++ld_stage == Smem::kStages) ld_stage = 0;
       ld_left -= kPagedWarps;
@@ -264,6 +289,20 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
 #pragma unroll
   for (int i = 0; i < Smem::kStages - 1; ++i) load();
 
+  // ---- what the lane reads of a tile: of keys, row g ^ 4 (g & 1) of a group of eight, chunks c (and c + 4); of values, rows 2 c and
+  // (2 c + 1) ^ 4, D / 8 columns
+  uint32_t k_at[D / 64], v_at[2];
+  {
+    const int key = g ^ ((g & 1) << 2);
+#pragma unroll
+    for (int hh = 0; hh < D / 64; ++hh) k_at[hh] = key * D + (D == 128 ? (c + 4 * hh) ^ key : c ^ (key >> 1)) * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = (2 * c + i) ^ (i << 2);
+      v_at[i] = row * D + (D == 128 ? (g ^ row) * 16 : ((g >> 1) ^ (row >> 1)) * 16 + (g & 1) * 8);
+    }
+  }
+
   // ---- segments
   uint32_t stage = 0;
   int turn = 0;  // tiles of the run in front of the segment, modulo the warps
@@ -273,17 +312,17 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
     const int j0 = seg.j, j1 = left < seg.tiles - j0 ? j0 + static_cast<int>(left) : seg.tiles;
     const int rows = seg.s.n * p.group, row0 = seg.rt * kRows;
 
-    // the lane's rows: their scaled queries in parts, and the keys they see
-    uint32_t qa[kSteps][4], qb[kStacked ? (kHalf ? kSteps : 1) : kSteps][4], qc[(!kStacked && kHalf) ? kSteps : 1][4];
-    float factor[kHalves];
-    int limit[kHalves];
+    // B of S^T: the lane has columns 16 (c + 4 hh) .. + 15 of row g of each tile, scaled by 2^up, which takes the row's largest element
+    // into [2^14, 2^15).  What it does with scores needs rows 2 c and 2 c + 1.
+    uint32_t qf[kN][kSteps][2];
+    float factor[kN][2];
+    int limit[kN][2];
 #pragma unroll
-    for (int r = 0; r < kHalves; ++r) {
-      const int row = row0 + g + 8 * r;
+    for (int n = 0; n < kN; ++n) {
+      const int row = row0 + 8 * n + g;
       const bool live = row < rows;
       const int tok = live ? fast_div(row, p.by_group) : 0, head = live ? row - tok * p.group : 0;
-      const T* src = static_cast<const T*>(p.q) + (seg.s.start + tok) * p.q_st + (seg.h * p.group + head) * p.q_sh;
-      limit[r] = live ? (p.causal ? min(seg.s.len, seg.s.pos0() + tok + 1) : seg.s.len) : 0;
+      const T* src = static_cast<const T*>(p.q) + (seg.s.start + tok) * p.q_st + (seg.h * p.group + head) * p.q_sh + 16 * c;
       float x[D / 64][16];
       float top = 0.f;
       bool finite = true;
@@ -292,7 +331,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
 #pragma unroll
         for (int e = 0; e < 16; e += 8) {
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (live) w = *reinterpret_cast<const uint4*>(src + 64 * hh + 16 * c + e);
+          if (live) w = *reinterpret_cast<const uint4*>(src + 64 * hh + e);
           Pack2<T>::unpack(w.x, x[hh][e], x[hh][e + 1]);
           Pack2<T>::unpack(w.y, x[hh][e + 2], x[hh][e + 3]);
           Pack2<T>::unpack(w.z, x[hh][e + 4], x[hh][e + 5]);
@@ -306,250 +345,189 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^up takes the largest element into (224, 448]; a row that holds an infinity or NaN is NaN
       int up = 0;
-      if (top > 0.f && top <= 3.402823466e38f) {
-        const int bits = __float_as_int(top);
-        up = 8 - ((bits >> 23) - 127) - ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
-        up = min(max(up, -120), 120);
-      }
+      if (top > 0.f && top <= 3.402823466e38f) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
       const float mul = __int_as_float((up + 127) << 23);
-      const unsigned votes = __ballot_sync(0xffffffffu, finite);
-      factor[r] = ((votes >> (lane & ~3)) & 15u) == 15u ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
+      const unsigned votes = __ballot_sync(0xffffffffu, finite);  // a row that holds an infinity or NaN is NaN
+      const float f = ((votes >> (lane & ~3)) & 15u) == 15u ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
+      for (int e = 0; e < 2; ++e) {
+        factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
+        const int r = row0 + 8 * n + 2 * c + e;
+        limit[n][e] = r >= rows ? 0 : p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(r, p.by_group) + 1) : seg.s.len;
+      }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float y[4];
+      for (int hh = 0; hh < D / 64; ++hh) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = x[st >> 1][8 * (st & 1) + 4 * half + e] * mul;
-          const uint32_t a = e4m3_part4(y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] *= kLow;
-          const uint32_t b = e4m3_part4(y);
-          const uint32_t d = e4m3_last(y[0], y[1]) | (e4m3_last(y[2], y[3]) << 16);
-          if constexpr (kStacked) {
-            qa[st][2 * half] = a;
-            qa[st][2 * half + 1] = b;
-            if constexpr (kHalf) {
-              qb[st][2 * half] = 0u;
-              qb[st][2 * half + 1] = d;
-            }
-          } else {
-            qa[st][2 * half + r] = a;
-            qb[st][2 * half + r] = b;
-            if constexpr (kHalf) qc[st][2 * half + r] = d;
-          }
-        }
+        for (int e = 0; e < 8; ++e) qf[n][4 * hh + (e >> 1)][e & 1] = Pack2<__half>::pack(x[hh][2 * e] * mul, x[hh][2 * e + 1] * mul);
       }
     }
     // keys that every live row sees: the first row's token sees least
     const int least = p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(row0, p.by_group) + 1) : seg.s.len;
 
-    float o[kCols][4];
+    float o[kN][kDims][4];
+    float m[kN][2], l[kN][2], v_ref = 0.f, to_ref = 0.f;  // O is in units of v_ref / kPUnit = 1 / to_ref
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[kHalves], l[kHalves], v_ref = 0.f;  // v_ref: O is in units of it / 256
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-    for (int r = 0; r < kHalves; ++r) {
-      m[r] = -INFINITY;
-      l[r] = 0.f;
+      for (int i = 0; i < kDims; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
     }
 
     for (int j = j0 + ((warp - turn) & (kPagedWarps - 1)); j < j1; j += kPagedWarps) {
       cp_async_wait<Smem::kStages - 2>();
       __syncwarp();  // every lane's copies are there, and every lane is done with the tile before: its stage is free
       load();
-      const uint8_t* tile = sm.ring[warp][stage];
-      const float ks[2] = {sm.scales[warp][stage][0], sm.scales[warp][stage][1]};
-      const float vs[2] = {sm.scales[warp][stage][2], sm.scales[warp][stage][3]};
+      const uint32_t tile = smem_u32(sm.ring[warp][stage]);
+      const float4 scales = *reinterpret_cast<const float4*>(sm.scales[warp][stage]);
 
-      // scores of the 32 keys: column n of group i is key 8 i + (n ^ 4 (n & 1))
-      float x[4][2 * kHalves];
+      // scores of the 32 keys: row r of half t is key 16 t + (r ^ 4 (r & 1)); the lane has rows g and g + 8, columns 2 c and 2 c + 1
+      float x[kN][2][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 8 * i + (g ^ ((g & 1) << 2));
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) x[n][t][0] = x[n][t][1] = x[n][t][2] = x[n][t][3] = 0.f;
 #pragma unroll
         for (int hh = 0; hh < D / 64; ++hh) {
-          const int chunk = c + 4 * hh;
-          const int sw = D == 128 ? chunk ^ (key & 7) : chunk ^ ((key >> 1) & 3);
-          const uint4 k4 = *reinterpret_cast<const uint4*>(tile + key * D + sw * 16);
-          const int st = 2 * hh;
-          mma_e4m3(s, qa[st][0], qa[st][1], qa[st][2], qa[st][3], k4.x, k4.y);
-          mma_e4m3(s, qa[st + 1][0], qa[st + 1][1], qa[st + 1][2], qa[st + 1][3], k4.z, k4.w);
-          if constexpr (!kStacked || kHalf) {
-            mma_e4m3(s, qb[st][0], qb[st][1], qb[st][2], qb[st][3], k4.x, k4.y);
-            mma_e4m3(s, qb[st + 1][0], qb[st + 1][1], qb[st + 1][2], qb[st + 1][3], k4.z, k4.w);
-          }
-          if constexpr (!kStacked && kHalf) {
-            mma_e4m3(s, qc[st][0], qc[st][1], qc[st][2], qc[st][3], k4.x, k4.y);
-            mma_e4m3(s, qc[st + 1][0], qc[st + 1][1], qc[st + 1][2], qc[st + 1][3], k4.z, k4.w);
-          }
-        }
-        if constexpr (kStacked) {
-          x[i][0] = s[0] + s[2] * (1.f / kLow);
-          x[i][1] = s[1] + s[3] * (1.f / kLow);
-        } else {
+          const uint4 ka = lds128(tile + k_at[hh] + 16 * t * D), kb = lds128(tile + k_at[hh] + (16 * t + 8) * D);
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][e] = s[e];
+          for (int w = 0; w < 4; ++w) {
+            uint32_t a0, a1, a2, a3;
+            codes_f16(wa[w], a0, a2);
+            codes_f16(wb[w], a1, a3);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma_f16(x[n][t], a0, a1, a2, a3, qf[n][4 * hh + w][0], qf[n][4 * hh + w][1]);
+          }
         }
       }
-      const bool masked = (j + 1) * kPagedTile > least || ks[0] == 0.f || ks[1] == 0.f;
-      float pv[2] = {0.f, 0.f};  // 256 vscale / v_ref of the halves
+      // keys that a row does not see, or that are not there
+      if ((j + 1) * kPagedTile > least || scales.x == 0.f || scales.y == 0.f) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const bool there = (t == 0 ? scales.x : scales.y) != 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = j * kPagedTile + 16 * t + 8 * (e >> 1) + (g ^ ((g & 1) << 2));
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+              if (!there || key >= limit[n][e & 1]) x[n][t][e] = -INFINITY;
+          }
+        }
+      }
+      bool moved = false;
       float shrink_o = 1.f;
-      {
-        const float top = fmaxf(vs[0], vs[1]);
-        if (top > v_ref) {
-          shrink_o = v_ref / top;  // powers of two (0 at first, where O is 0)
-          v_ref = top;
-        }
-        if (v_ref > 0.f) {
-          pv[0] = 256.f * (vs[0] / v_ref);
-          pv[1] = 256.f * (vs[1] / v_ref);
-        }
+      if (fmaxf(scales.z, scales.w) > v_ref) {  // powers of two; 0 at first, where O is 0
+        const float top = fmaxf(scales.z, scales.w);
+        shrink_o = v_ref / top;
+        v_ref = top;
+        to_ref = kPUnit / top;
+        moved = true;
       }
-      bool moved = shrink_o != 1.f;
-      float alpha[kHalves];
+      const __half2 pv[2] = {__float2half2_rn(scales.z * to_ref), __float2half2_rn(scales.w * to_ref)};  // at most kPUnit
+      float alpha[kN][2];
+      uint32_t pb[kN][2][2];  // P' as B of O^T
 #pragma unroll
-      for (int r = 0; r < kHalves; ++r) {
-        float top = -INFINITY;
+      for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float f = factor[r] * ks[i >> 1];
+        for (int e = 0; e < 2; ++e) {
+          // not 0 (a page without a scale, or less than fp32 holds): -inf has to stay it
+          float f0 = factor[n][e] * scales.x, f1 = factor[n][e] * scales.y;
+          f0 = f0 == 0.f ? 1.17549435e-38f : f0;
+          f1 = f1 == 0.f ? 1.17549435e-38f : f1;
+          float top = fmaxf(fmaxf(x[n][0][e], x[n][0][2 + e]) * f0, fmaxf(x[n][1][e], x[n][1][2 + e]) * f1);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const bool adopt = top > m[n][e] + kGrowth;  // of -inf: any maximum
+          alpha[n][e] = adopt ? fast_exp2(m[n][e] - top) : 1.f;
+          moved = moved || adopt;
+          m[n][e] = adopt ? top : m[n][e];
+          const float m_safe = m[n][e] == -INFINITY ? 0.f : m[n][e];
+          x[n][0][e] = fast_exp2(fmaf(x[n][0][e], f0, -m_safe));
+          x[n][0][2 + e] = fast_exp2(fmaf(x[n][0][2 + e], f0, -m_safe));
+          x[n][1][e] = fast_exp2(fmaf(x[n][1][e], f1, -m_safe));
+          x[n][1][2 + e] = fast_exp2(fmaf(x[n][1][2 + e], f1, -m_safe));
+          l[n][e] = fmaf(l[n][e], alpha[n][e], (x[n][0][e] + x[n][0][2 + e]) + (x[n][1][e] + x[n][1][2 + e]));
+        }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& s = x[i][2 * r + e];
-            s *= f;
-            if (masked) {
-              const int n = 2 * c + e, key = j * kPagedTile + 8 * i + (n ^ (e << 2));
-              if (key >= limit[r] || ks[i >> 1] == 0.f) s = -INFINITY;
-            }
-            top = fmaxf(top, s);
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const __half2 y = __hmul2(__floats2half2_rn(x[n][t][2 * h], x[n][t][2 * h + 1]), pv[t]);
+            pb[n][t][h] = movmatrix(*reinterpret_cast<const uint32_t*>(&y));
           }
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m_new = fmaxf(m[r], top);
-        const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-        alpha[r] = fast_exp2(m[r] - m_safe);  // 0 while m is -inf, as O and l are
-        moved = moved || (m_new != m[r]);
-        m[r] = m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& s = x[i][2 * r + e];
-            s = fast_exp2(s - m_safe);
-            sum += s;
-            s *= pv[i >> 1];
-          }
-        }
-        l[r] = l[r] * alpha[r] + sum;
       }
       if (__any_sync(0xffffffffu, moved)) {
-        const float f0 = alpha[0] * shrink_o, f1 = (kStacked ? alpha[0] : alpha[kHalves - 1]) * shrink_o;
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) {
-          o[i][0] *= f0;
-          o[i][1] *= f0;
-          o[i][2] *= f1;
-          o[i][3] *= f1;
-        }
-      }
-      // P in parts, as A: columns 4 c .. of the first 16 keys are columns 2 c, 2 c + 1 of score groups 0 and 1
-      uint32_t pa[4], pb[4];
+        for (int n = 0; n < kN; ++n) {
+          const float f0 = alpha[n][0] * shrink_o, f1 = alpha[n][1] * shrink_o;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int r = 0; r < kHalves; ++r) {
-          float y[4] = {x[2 * half][2 * r], x[2 * half][2 * r + 1], x[2 * half + 1][2 * r], x[2 * half + 1][2 * r + 1]};
-          const uint32_t a = e4m3_part4(y);
-          const uint32_t b = e4m3_last(y[0] * kLow, y[1] * kLow) | (e4m3_last(y[2] * kLow, y[3] * kLow) << 16);
-          if constexpr (kStacked) {
-            pa[2 * half] = a;
-            pa[2 * half + 1] = b;
-          } else {
-            pa[2 * half + r] = a;
-            pb[2 * half + r] = b;
+          for (int i = 0; i < kDims; ++i) {
+            o[n][i][0] *= f0;
+            o[n][i][1] *= f1;
+            o[n][i][2] *= f0;
+            o[n][i][3] *= f1;
           }
         }
       }
-      // O += P V: the lane's value rows are keys 2 c, (2 c + 1) ^ 4, and those plus 8 of either half; its columns D / 8 from D / 8 g on
-      constexpr int kWords = D / 32;  // of 4 columns
-      uint32_t vw[2][4][kWords];
+      // O^T += V^T P'^T: of half t the lane has value rows 2 c, (2 c + 1) ^ 4 and those plus 8, columns D / 8 from D / 8 g on: rows g and
+      // g + 8 of tile i are columns 2 i and 2 i + 1 of them
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int t = 0; t < 2; ++t) {
+        constexpr int kWords = D / 32;  // of 4 columns
+        uint32_t vw[4][kWords];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int n = 2 * c + (i & 1);
-          const int key = 16 * half + 8 * (i >> 1) + (n ^ ((i & 1) << 2));
-          const uint8_t* row = tile + Smem::kTileBytes + key * D;
+          const uint32_t at = tile + Smem::kTileBytes + (16 * t + 8 * (i >> 1)) * D + v_at[i & 1];
           if constexpr (D == 128) {
-            const uint4 w = *reinterpret_cast<const uint4*>(row + ((g ^ (key & 7)) * 16));
-            vw[half][i][0] = w.x;
-            vw[half][i][1] = w.y;
-            vw[half][i][2] = w.z;
-            vw[half][i][3] = w.w;
+            const uint4 w = lds128(at);
+            vw[i][0] = w.x;
+            vw[i][1] = w.y;
+            vw[i][2] = w.z;
+            vw[i][3] = w.w;
           } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(row + (((g >> 1) ^ ((key >> 1) & 3)) * 16) + (g & 1) * 8);
-            vw[half][i][0] = w.x;
-            vw[half][i][1] = w.y;
+            const uint2 w = lds64(at);
+            vw[i][0] = w.x;
+            vw[i][1] = w.y;
           }
         }
-      }
 #pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        uint32_t b[2][4];
+        for (int w = 0; w < kWords; ++w) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t t0 = __byte_perm(vw[half][0][w], vw[half][1][w], 0x5140), t1 = __byte_perm(vw[half][2][w], vw[half][3][w], 0x5140);
-          const uint32_t t2 = __byte_perm(vw[half][0][w], vw[half][1][w], 0x7362), t3 = __byte_perm(vw[half][2][w], vw[half][3][w], 0x7362);
-          b[half][0] = __byte_perm(t0, t1, 0x5410);
-          b[half][1] = __byte_perm(t0, t1, 0x7632);
-          b[half][2] = __byte_perm(t2, t3, 0x5410);
-          b[half][3] = __byte_perm(t2, t3, 0x7632);
-        }
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t pick = half == 0 ? 0x5140u : 0x7362u;
+            uint32_t a0, a1, a2, a3;
+            codes_f16(__byte_perm(vw[0][w], vw[1][w], pick), a0, a1);
+            codes_f16(__byte_perm(vw[2][w], vw[3][w], pick), a2, a3);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          mma_e4m3(o[4 * w + e], pa[0], pa[1], pa[2], pa[3], b[0][e], b[1][e]);
-          if constexpr (!kStacked) mma_e4m3(o[4 * w + e], pb[0], pb[1], pb[2], pb[3], b[0][e], b[1][e]);
+            for (int n = 0; n < kN; ++n) mma_f16(o[n][2 * w + half], a0, a1, a2, a3, pb[n][t][0], pb[n][t][1]);
+          }
         }
       }
       if (++stage == Smem::kStages) stage = 0;
     }
 
     // ---- the warps' results meet
-    const float unit = v_ref * (1.f / 256.f);
+    const float unit = v_ref * (1.f / kPUnit);
 #pragma unroll
-    for (int r = 0; r < kHalves; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (c == 0) {
-        sm.ml[warp][0][g + 8 * r] = m[r];
-        sm.ml[warp][1][g + 8 * r] = l[r];
-      }
-    }
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w) {
-#pragma unroll
-      for (int e2 = 0; e2 < 2; ++e2) {  // columns n = 2 c + e2: D / 8 n + 4 w + 0 .. 3
-        const int col = (D / 8) * (2 * c + e2) + 4 * w;
-        if constexpr (kStacked) {
-          float4 y;
-          y.x = (o[4 * w][e2] + o[4 * w][2 + e2] * (1.f / kLow)) * unit;
-          y.y = (o[4 * w + 1][e2] + o[4 * w + 1][2 + e2] * (1.f / kLow)) * unit;
-          y.z = (o[4 * w + 2][e2] + o[4 * w + 2][2 + e2] * (1.f / kLow)) * unit;
-          y.w = (o[4 * w + 3][e2] + o[4 * w + 3][2 + e2] * (1.f / kLow)) * unit;
-          *reinterpret_cast<float4*>(&sm.o[warp][g][col]) = y;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-            *reinterpret_cast<float4*>(&sm.o[warp][g + 8 * r][col]) =
-                make_float4(o[4 * w][2 * r + e2] * unit, o[4 * w + 1][2 * r + e2] * unit, o[4 * w + 2][2 * r + e2] * unit,
-                            o[4 * w + 3][2 * r + e2] * unit);
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[n][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) {
+          sm.ml[warp][0][8 * n + 2 * c + e] = m[n][e];
+          sm.ml[warp][1][8 * n + 2 * c + e] = sum;
         }
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w)
+          *reinterpret_cast<float4*>(&sm.o[warp][8 * n + 2 * c + e][(D / 8) * g + 4 * w]) =
+              make_float4(o[n][2 * w][e] * unit, o[n][2 * w][2 + e] * unit, o[n][2 * w + 1][e] * unit, o[n][2 * w + 1][2 + e] * unit);
       }
     }
     __syncthreads();
