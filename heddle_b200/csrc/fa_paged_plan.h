@@ -22,8 +22,13 @@ HB_HD int paged_runs(long long total, int blocks) {
   const long long most = (total + kPagedWarps - 1) / kPagedWarps;
   return static_cast<int>(most < blocks ? (most < 1 ? 1 : most) : blocks);
 }
+// a / b; 32-bit where both fit, which takes a fraction of the time
+HB_HD long long paged_div(long long a, int b) {
+  return (a >> 31) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
 HB_HD long long paged_begin(long long total, int runs, int w) {  // total < 2^48, runs < 2^12
-  return total / runs * w + total % runs * w / runs;
+  const long long per = paged_div(total, runs);
+  return per * w + paged_div((total - per * runs) * w, runs);
 }
 // The run of tile t: the last w with begin(w) = floor(w total / runs) <= t.
 HB_HD int paged_run_of(long long total, int runs, long long t) { return static_cast<int>(((t + 1) * runs - 1) / total); }

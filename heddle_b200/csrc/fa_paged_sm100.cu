@@ -40,8 +40,14 @@ static int64_t paged_most_rows(const hb_fa_paged_args* a) {
 }
 static int paged_tile_rows(const hb_fa_paged_args* a) { return paged_most_rows(a) <= 8 ? 8 : kPagedMaxRows; }
 
+static int paged_blocks(const hb_fa_paged_args* a, int sm_count) {
+  const bool few = paged_tile_rows(a) == 8;
+  return sm_count * (a->cache.D == 128 ? (few ? paged_blocks_per_sm<128, 8> : paged_blocks_per_sm<128, 16>)
+                                       : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
+}
+
 static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
-  const uint64_t blocks = 2ull * sm_count, rows = paged_tile_rows(a);
+  const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
   return 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
 }
 
@@ -60,11 +66,15 @@ static int launch_rows(const FaPagedParams& p, int blocks, cudaStream_t stream) 
     }
   }
   HB_CUDA_CHECK(launch_dependent(kernel, blocks, kPagedThreads, sizeof(Smem), stream, 0, p));
-  // an item of few has parts in many runs: a warp of the merge for every four
+  // parts of an item at most: a warp of the merge for every four
   const long long items = static_cast<long long>(p.c.B) * p.c.Hkv;
   const long long parts = (blocks + items - 1) / items + 1;
-  const unsigned warps = static_cast<unsigned>(std::min<long long>(kPagedCombineWarps, (parts + 3) / 4));
-  HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D>, blocks * kRows, 32 * warps, 0, stream, 0, p, kRows));
+  if (parts <= 8) {
+    HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, true>, blocks * kRows / 8, 32 * 8, 0, stream, 0, p, kRows));
+  } else {
+    const unsigned warps = static_cast<unsigned>(std::min<long long>(kPagedCombineWarps, (parts + 3) / 4));
+    HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, false>, blocks * kRows, 32 * warps, 0, stream, 0, p, kRows));
+  }
   return HB_OK;
 }
 template <typename T>
@@ -105,7 +115,7 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
                      (unsigned long long)(workspace == nullptr ? 0 : bytes));
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return set_error(HB_ERR_ALIGN, "hb_fa_paged: the workspace must be 16-byte aligned");
   const hb_kv_cache& c = a->cache;
-  const int rows = paged_tile_rows(a), blocks = 2 * st->sm_count;
+  const int rows = paged_tile_rows(a), blocks = paged_blocks(a, st->sm_count);
   FaPagedParams p;
   p.c = kv_view(c, st);
   p.q = a->q;

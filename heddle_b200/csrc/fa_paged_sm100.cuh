@@ -50,13 +50,19 @@ struct FaPagedParams {
   PagedHead* heads; // [blocks]
 };
 
+// Blocks an SM holds: what bounds a warp is the latency of its own instructions (four cycles and a half each with two warps to a
+// scheduler), so registers and the ring are cut to fit as many warps as do not spill.
+template <int D, int kRows>
+constexpr int paged_blocks_per_sm = D == 128 ? (kRows == 8 ? 3 : 2) : (kRows == 8 ? 4 : 3);
+
 template <int D, int kRows>
 struct FaPagedSmem {
   static constexpr int kTileBytes = kPagedTile * D;  // of keys, and of values
-  static constexpr int kStages = D == 128 ? (kRows == 8 ? 3 : 2) : (kRows == 8 ? 6 : 4);
+  static constexpr int kStages = D == 128 ? (kRows == 8 ? 2 : 3) : 3;
+  static constexpr int kFrags = kRows / 8 * (D / 16);  // accumulator tiles of O^T
   alignas(128) uint8_t ring[kPagedWarps][kStages][2 * kTileBytes];
-  float o[kPagedWarps][kRows][D];
-  float ml[kPagedWarps][2][kRows];
+  float4 o[kPagedWarps / 2][kFrags][32];   // a warp's accumulators, as its lanes hold them ...
+  float ml[kPagedWarps / 2][2][kRows];     // ... and its maxima and sums
   alignas(16) float scales[kPagedWarps][kStages][4];  // keys, values of the tile's two halves; 0: a page that the cache does not have
   long long sums[kPagedWarps];
   long long found_at;
@@ -134,7 +140,7 @@ __device__ __forceinline__ void paged_next_item(const FaPagedParams& p, PagedCur
 }
 
 template <typename T, int D, int kRows>
-__global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const __grid_constant__ FaPagedParams p) {
+__global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)) fa_paged_rows_kernel(const __grid_constant__ FaPagedParams p) {
   using Smem = FaPagedSmem<D, kRows>;
   constexpr int kSteps = D / 16;  // products along head_dim
   constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
@@ -144,54 +150,69 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const KvView& kv = p.c;
-  grid_launch_dependents();
   grid_wait();
 
-  // ---- this block's run of the list
-  long long mine = 0;
-  for (int b = threadIdx.x; b < kv.B; b += kPagedThreads) {
-    int tiles, row_tiles;
-    mine += paged_list(p, kv_seq(kv, b), kRows, tiles, row_tiles);
-    if (blockIdx.x == 0) {
-      const uint32_t f = kv_seq_faults(kv, b);
-      if (f != 0) kv_report(kv, f);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sm.sums[warp] = mine;
-  if (threadIdx.x == 0) p.heads[blockIdx.x].last = -1;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < kPagedWarps; ++w) total += sm.sums[w];
-  if (total == 0) return;
-  const int runs = paged_runs(total, gridDim.x), run = blockIdx.x;
-  if (run >= runs) return;
-  const long long begin = paged_begin(total, runs, run), end = paged_begin(total, runs, run + 1);
-  long long before = 0;  // of the sequences in front of this round's
-  for (int b0 = 0; b0 < kv.B && before <= begin; b0 += kPagedThreads) {
+  // ---- this block's run of the list: the sequences' parts are added up in rounds of a block's threads
+  long long total = 0, own = 0, upto = 0;  // own: of the last round
+  for (int b0 = 0; b0 < kv.B; b0 += kPagedThreads) {
     const int b = b0 + threadIdx.x;
     int tiles, row_tiles;
-    const long long own = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, tiles, row_tiles) : 0;
-    long long upto = own;
+    own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, tiles, row_tiles) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += up;
     }
-    __syncthreads();
+    if (b0 > 0) __syncthreads();
     if (lane == 31) sm.sums[warp] = upto;
     __syncthreads();
-    long long at = before;
+    upto += total;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) {
-      if (w < warp) at += sm.sums[w];
-      before += sm.sums[w];
+      if (w < warp) upto += sm.sums[w];
+      total += sm.sums[w];
     }
-    if (at + upto > begin && at + upto - own <= begin) {
-      sm.found = b;
-      sm.found_at = at + upto - own;
+  }
+  const int run = blockIdx.x;
+  if (threadIdx.x == 0) p.heads[run].last = -1;
+  if (run == 0) {
+    for (int b = threadIdx.x; b < kv.B; b += kPagedThreads) {
+      const uint32_t f = kv_seq_faults(kv, b);
+      if (f != 0) kv_report(kv, f);
+    }
+  }
+  const int runs = paged_runs(total, gridDim.x);
+  if (total == 0 || run >= runs) return;
+  const long long begin = paged_begin(total, runs, run), end = paged_begin(total, runs, run + 1);
+  if (kv.B <= kPagedThreads) {
+    if (upto > begin && upto - own <= begin) {
+      sm.found = threadIdx.x;
+      sm.found_at = upto - own;
+    }
+  } else {
+    long long before = 0;  // of the sequences in front of this round's
+    for (int b0 = 0; b0 < kv.B && before <= begin; b0 += kPagedThreads) {
+      const int b = b0 + threadIdx.x;
+      int tiles, row_tiles;
+      own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, tiles, row_tiles) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      __syncthreads();
+      if (lane == 31) sm.sums[warp] = upto;
+      __syncthreads();
+      upto += before;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        if (w < warp) upto += sm.sums[w];
+        before += sm.sums[w];
+      }
+      if (upto > begin && upto - own <= begin) {
+        sm.found = b;
+        sm.found_at = upto - own;
+      }
     }
   }
   __syncthreads();
@@ -200,10 +221,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
   seg.b = sm.found;
   paged_enter(p, seg, kRows);
   {
-    const long long in = begin - sm.found_at;
-    const long long item = in / seg.tiles;
+    const long long in = begin - sm.found_at, item = paged_div(in, seg.tiles);
     seg.j = static_cast<int>(in - item * seg.tiles);
-    seg.h = static_cast<int>(item / seg.row_tiles);
+    seg.h = static_cast<int>(paged_div(item, seg.row_tiles));
     seg.rt = static_cast<int>(item - static_cast<long long>(seg.h) * seg.row_tiles);
   }
 
@@ -239,9 +259,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
     const int row = i * kRowsAtOnce + ld_row, chunk = lane % kChunks;
     ld_dst[i] = row * D + (D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) * 16;
   }
-  const uint8_t* const ld_k = kv.k + ld_row * kv.k_ss + lane % kChunks * 16;
-  const uint8_t* const ld_v = kv.v + ld_row * kv.v_ss + lane % kChunks * 16;
-  const long long k_step = kRowsAtOnce * kv.k_ss, v_step = kRowsAtOnce * kv.v_ss;
+  const uint8_t* const ld_k = kv.k + kv_offset(ld_row, kv.k_ss) + lane % kChunks * 16;
+  const uint8_t* const ld_v = kv.v + kv_offset(ld_row, kv.v_ss) + lane % kChunks * 16;
+  const long long k_step = kv_offset(kRowsAtOnce, kv.k_ss), v_step = kv_offset(kRowsAtOnce, kv.v_ss);
   auto load = [&]() {  // one tile, or nothing behind the run's end: a group of copies either way
     if (ld_left > 0) {
       const int tok = ld.j * kPagedTile;
@@ -252,8 +272,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
       for (int half = 0; half < 2; ++half) {
         const int page = half == 0 ? page0 : page1;
         const int place = half == 0 ? at : (kv.page_shift == 4 ? 0 : at + 16);
-        const uint8_t* ks = ld_k + page * kv.k_sp + ld.h * kv.k_sh + place * kv.k_ss;
-        const uint8_t* vs = ld_v + page * kv.v_sp + ld.h * kv.v_sh + place * kv.v_ss;
+        const uint8_t* ks = ld_k + kv_offset(page, kv.k_sp) + kv_offset(ld.h, kv.k_sh) + kv_offset(place, kv.k_ss);
+        const uint8_t* vs = ld_v + kv_offset(page, kv.v_sp) + kv_offset(ld.h, kv.v_sh) + kv_offset(place, kv.v_ss);
         if (full) {
 #pragma unroll
           for (int i = 0; i < kCopies; ++i, ks += k_step, vs += v_step) {
@@ -510,69 +530,103 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
       if (++stage == Smem::kStages) stage = 0;
     }
 
-    // ---- the warps' results meet
-    const float unit = v_ref * (1.f / kPUnit);
+    // ---- the warps' results meet: 2 and 3 hand theirs to 0 and 1, 1 to 0, which stores the rows
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float sum = l[n][e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        if (g == 0) {
-          sm.ml[warp][0][8 * n + 2 * c + e] = m[n][e];
-          sm.ml[warp][1][8 * n + 2 * c + e] = sum;
-        }
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w)
-          *reinterpret_cast<float4*>(&sm.o[warp][8 * n + 2 * c + e][(D / 8) * g + 4 * w]) =
-              make_float4(o[n][2 * w][e] * unit, o[n][2 * w][2 + e] * unit, o[n][2 * w + 1][e] * unit, o[n][2 * w + 1][2 + e] * unit);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
       }
     }
-    __syncthreads();
-    const bool whole = j0 == 0 && j1 == seg.tiles;
-    const int slot = 2 * run + (first ? 0 : 1);
-    for (int i = threadIdx.x; i < kRows * (D / 8); i += kPagedThreads) {
-      const int r = i / (D / 8), col = i % (D / 8) * 8, row = row0 + r;
-      if (row >= rows) continue;
-      float top = sm.ml[0][0][r];
+    const float unit = v_ref * (1.f / kPUnit);
 #pragma unroll
-      for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm.ml[w][0][r]);
-      const float safe = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, y[8] = {};
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const float wt = fast_exp2(sm.ml[w][0][r] - safe);
-        sum += wt * sm.ml[w][1][r];
+      for (int i = 0; i < kDims; ++i) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const float4 z = *reinterpret_cast<const float4*>(&sm.o[w][r][col + e]);
-          y[e] += wt * z.x;
-          y[e + 1] += wt * z.y;
-          y[e + 2] += wt * z.z;
-          y[e + 3] += wt * z.w;
+        for (int e = 0; e < 4; ++e) o[n][i][e] *= unit;
+      }
+    }
+    auto give = [&](int slot) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int i = 0; i < kDims; ++i) sm.o[slot][n * kDims + i][lane] = make_float4(o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
+        if (g == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sm.ml[slot][0][8 * n + 2 * c + e] = m[n][e];
+            sm.ml[slot][1][8 * n + 2 * c + e] = l[n][e];
+          }
         }
       }
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;  // a row without keys is 0, one with a NaN is NaN
+    };
+    auto take = [&](int slot) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= inv;
-      const float lse2 = sum != 0.f ? safe + fast_log2(sum) : -INFINITY;
-      if (whole) {
-        const int tok = fast_div(row, p.by_group), head = seg.h * p.group + row - tok * p.group;
-        T* dst = static_cast<T*>(p.o) + (seg.s.start + tok) * p.o_st + head * p.o_sh + col;
-        uint4 w4;
-        w4.x = Pack2<T>::pack(y[0], y[1]);
-        w4.y = Pack2<T>::pack(y[2], y[3]);
-        w4.z = Pack2<T>::pack(y[4], y[5]);
-        w4.w = Pack2<T>::pack(y[6], y[7]);
-        *reinterpret_cast<uint4*>(dst) = w4;
-        if (col == 0 && p.lse != nullptr) p.lse[static_cast<long long>(seg.s.start + tok) * p.Hq + head] = lse2 * 0.6931471805599453f;
-      } else {
-        float* dst = p.part_o + (static_cast<long long>(slot) * kRows + r) * D + col;
-        *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
-        if (col == 0) p.part_lse[static_cast<long long>(slot) * kRows + r] = lse2;
+      for (int n = 0; n < kN; ++n) {
+        float w0[2], w1[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float other = sm.ml[slot][0][8 * n + 2 * c + e], top = fmaxf(m[n][e], other), safe = top == -INFINITY ? 0.f : top;
+          w0[e] = fast_exp2(m[n][e] - safe);
+          w1[e] = fast_exp2(other - safe);
+          l[n][e] = w0[e] * l[n][e] + w1[e] * sm.ml[slot][1][8 * n + 2 * c + e];
+          m[n][e] = top;
+        }
+#pragma unroll
+        for (int i = 0; i < kDims; ++i) {
+          const float4 y = sm.o[slot][n * kDims + i][lane];
+          o[n][i][0] = w0[0] * o[n][i][0] + w1[0] * y.x;
+          o[n][i][1] = w0[1] * o[n][i][1] + w1[1] * y.y;
+          o[n][i][2] = w0[0] * o[n][i][2] + w1[0] * y.z;
+          o[n][i][3] = w0[1] * o[n][i][3] + w1[1] * y.w;
+        }
+      }
+    };
+    const bool whole = j0 == 0 && j1 == seg.tiles;
+    const int slot = 2 * run + (first ? 0 : 1);
+    if (warp >= 2) give(warp - 2);
+    __syncthreads();
+    if (warp < 2) take(warp);
+    if (warp == 1) {
+      __syncwarp();
+      give(1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      take(1);
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * n + 2 * c + e, row = row0 + r;
+          if (row >= rows) continue;
+          const float sum = l[n][e], inv = sum != 0.f ? 1.f / sum : 0.f;  // a row without keys is 0, one with a NaN is NaN
+          const float lse2 = sum != 0.f ? (m[n][e] == -INFINITY ? 0.f : m[n][e]) + fast_log2(sum) : -INFINITY;
+          if (whole) {
+            const int tok = fast_div(row, p.by_group), head = seg.h * p.group + row - tok * p.group;
+            T* dst = static_cast<T*>(p.o) + (seg.s.start + tok) * p.o_st + head * p.o_sh + (D / 8) * g;
+#pragma unroll
+            for (int i = 0; i < kDims; i += 4) {  // 8 columns; rows g, g + 8 of tile i are columns 2 i, 2 i + 1
+              uint4 y;
+              y.x = Pack2<T>::pack(o[n][i][e] * inv, o[n][i][2 + e] * inv);
+              y.y = Pack2<T>::pack(o[n][i + 1][e] * inv, o[n][i + 1][2 + e] * inv);
+              y.z = Pack2<T>::pack(o[n][i + 2][e] * inv, o[n][i + 2][2 + e] * inv);
+              y.w = Pack2<T>::pack(o[n][i + 3][e] * inv, o[n][i + 3][2 + e] * inv);
+              *reinterpret_cast<uint4*>(dst + 2 * i) = y;
+            }
+            if (g == 0 && p.lse != nullptr) p.lse[static_cast<long long>(seg.s.start + tok) * p.Hq + head] = lse2 * 0.6931471805599453f;
+          } else {
+            float* dst = p.part_o + (static_cast<long long>(slot) * kRows + r) * D + (D / 8) * g;
+#pragma unroll
+            for (int i = 0; i < kDims; i += 2)
+              *reinterpret_cast<float4*>(dst + 2 * i) =
+                  make_float4(o[n][i][e] * inv, o[n][i][2 + e] * inv, o[n][i + 1][e] * inv, o[n][i + 1][2 + e] * inv);
+            if (g == 0) p.part_lse[static_cast<long long>(slot) * kRows + r] = lse2;
+          }
+        }
       }
     }
     if (threadIdx.x == 0 && j0 == 0 && !whole) {
@@ -591,22 +645,24 @@ __global__ void __launch_bounds__(kPagedThreads, 2) fa_paged_rows_kernel(const _
     if (t < end) paged_next_item(p, seg, kRows);
   }
   cp_async_wait<0>();
+  grid_launch_dependents();
 }
 
-// Merges the parts of an item: one block per (run that starts an item in parts, row); its warps deal the parts out, a lane has
-// D / 32 columns; weights 2^(lse - max).
+// Merges the parts of an item, a row a warp-group: its warps deal the parts out, a lane has D / 32 columns; weights 2^(lse - max).  Where
+// items are in many parts a block has one row, and a warp for every four parts; elsewhere a warp goes over its row's parts alone,
+// and a block has a row for every warp: a decode step of many sequences has a few hundred items in parts, not thousands of blocks.
 constexpr int kPagedCombineWarps = 8;
-template <typename T, int D>
+template <typename T, int D, bool kAlone>
 __global__ void __launch_bounds__(32 * kPagedCombineWarps) fa_paged_combine_kernel(const __grid_constant__ FaPagedParams p, int kRows) {
-  grid_launch_dependents();
   grid_wait();
-  const int run = blockIdx.x / kRows, r = blockIdx.x - run * kRows;
+  const int warp = kAlone ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kAlone ? 1 : blockDim.x >> 5;
+  const int work = kAlone ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
+  const int run = work / kRows, r = work - run * kRows;
   const PagedHead hd = p.heads[run];
   if (hd.last < 0) return;
   const KvSeq s = kv_seq(p.c, hd.b);
   const int row = hd.rt * kRows + r;
   if (row >= s.n * p.group) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   auto slot_of = [&](int w) -> long long { return w == run ? hd.slot : 2 * w; };
 
   float top = -INFINITY;
@@ -635,25 +691,23 @@ __global__ void __launch_bounds__(32 * kPagedCombineWarps) fa_paged_combine_kern
       acc[1] += wt * x.y;
     }
   }
-  __shared__ float s_acc[kPagedCombineWarps][D], s_sum[kPagedCombineWarps];
+  if constexpr (!kAlone) {
+    __shared__ float s_acc[kPagedCombineWarps][D], s_sum[kPagedCombineWarps];
 #pragma unroll
-  for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  if (warp != 0) return;
-  sum = 0.f;
-  for (int k = 0; k < warps; ++k) sum += s_sum[k];
+    for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int k = 1; k < warps; ++k) {
+      sum += s_sum[k];
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) acc[e] += s_acc[k][lane * kCols + e];
+    }
+  }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   uint32_t packed[kCols / 2];
 #pragma unroll
-  for (int e = 0; e < kCols; e += 2) {
-    float a = 0.f, b = 0.f;
-    for (int k = 0; k < warps; ++k) {
-      a += s_acc[k][lane * kCols + e];
-      b += s_acc[k][lane * kCols + e + 1];
-    }
-    packed[e / 2] = Pack2<T>::pack(a * inv, b * inv);
-  }
+  for (int e = 0; e < kCols; e += 2) packed[e / 2] = Pack2<T>::pack(acc[e] * inv, acc[e + 1] * inv);
   const int tok = fast_div(row, p.by_group), head = hd.h * p.group + row - tok * p.group;
   T* dst = static_cast<T*>(p.o) + (s.start + tok) * p.o_st + head * p.o_sh + lane * kCols;
   if constexpr (kCols == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);

@@ -257,12 +257,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     c.k_scale[scale_at] = k_new;
     c.v_scale[scale_at] = v_new;
   }
-  uint8_t* kp = c.k + page * c.k_sp + h * c.k_sh;
-  uint8_t* vp = c.v + page * c.v_sp + h * c.v_sh;
-  auto shrink = [&](uint8_t* base, long long stride, float factor) {
+  uint8_t* kp = c.k + kv_offset(page, c.k_sp) + kv_offset(h, c.k_sh);
+  uint8_t* vp = c.v + kv_offset(page, c.v_sp) + kv_offset(h, c.v_sh);
+  auto shrink = [&](uint8_t* base, unsigned stride, float factor) {
     const __half2 f = __float2half2_rn(factor);
     for (int i = tid; i < earlier * kPieces; i += GS) {
-      uint4* at = reinterpret_cast<uint4*>(base + (i / kPieces) * stride + piece * 16);
+      uint4* at = reinterpret_cast<uint4*>(base + kv_offset(i / kPieces, stride) + piece * 16);
       uint4 w = *at;
       w.x = append_shrink(w.x, f);
       w.y = append_shrink(w.y, f);
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     const bool live = i0 + tid < total;
     const bool finite = load(i0 + tid, live, x, y);
     if (!live) continue;
-    const long long place = earlier + (i0 + tid) / kPieces;
+    const int place = earlier + (i0 + tid) / kPieces;
     uint2 lo = make_uint2(append_codes4(x, k_inv), append_codes4(x + 4, k_inv));
     uint2 hi = make_uint2(append_codes4(x + 8, k_inv), append_codes4(x + 12, k_inv));
     uint4 val = make_uint4(append_codes4(y, v_inv), append_codes4(y + 4, v_inv), append_codes4(y + 8, v_inv), append_codes4(y + 12, v_inv));
@@ -286,9 +286,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
       lo = hi = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
       val = make_uint4(0u, 0u, 0u, 0u);
     }
-    *reinterpret_cast<uint2*>(kp + place * c.k_ss + piece * 8) = lo;
-    *reinterpret_cast<uint2*>(kp + place * c.k_ss + D / 2 + piece * 8) = hi;
-    *reinterpret_cast<uint4*>(vp + place * c.v_ss + piece * 16) = val;
+    *reinterpret_cast<uint2*>(kp + kv_offset(place, c.k_ss) + piece * 8) = lo;
+    *reinterpret_cast<uint2*>(kp + kv_offset(place, c.k_ss) + D / 2 + piece * 8) = hi;
+    *reinterpret_cast<uint4*>(vp + kv_offset(place, c.v_ss) + piece * 16) = val;
   }
 }
 

@@ -1,6 +1,8 @@
 // The paged key/value cache as its kernels see it (hb_kv_cache in the C ABI): checks on the host, sequences and pages on the device.
 #pragma once
 
+#include <initializer_list>
+
 #include "host_common.h"
 
 namespace hb {
@@ -10,7 +12,7 @@ struct KvView {
   uint8_t* v;
   float* k_scale;
   float* v_scale;
-  long long k_sp, k_sh, k_ss, v_sp, v_sh, v_ss;
+  unsigned k_sp, k_sh, k_ss, v_sp, v_sh, v_ss;  // strides of pages, heads and tokens
   const int* table;
   const int* lens;
   const int* starts;  // nullptr: `each` rows a sequence
@@ -37,6 +39,8 @@ inline int kv_cache_check(const char* fn, const hb_kv_cache& c, bool* empty) {
   }
   if (c.page_table == nullptr || c.seq_lens == nullptr || c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr)
     return set_error(HB_ERR_BAD_ARG, "%s: NULL cache pointer", fn);
+  for (int64_t s : {c.k_stride_p, c.k_stride_h, c.k_stride_s, c.v_stride_p, c.v_stride_h, c.v_stride_s})
+    if (s < 0 || s > 0xffffffffll) return set_error(HB_ERR_UNSUPPORTED, "%s: strides of the pages must be within 0 .. 2^32 - 1", fn);
   const uintptr_t words = reinterpret_cast<uintptr_t>(c.page_table) | reinterpret_cast<uintptr_t>(c.seq_lens) |
                           reinterpret_cast<uintptr_t>(c.starts) | reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale);
   const uint64_t rows = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | static_cast<uint64_t>(c.k_stride_p) |
@@ -53,12 +57,12 @@ inline KvView kv_view(const hb_kv_cache& c, const DeviceState* st) {
   v.v = static_cast<uint8_t*>(c.v);
   v.k_scale = c.k_scale;
   v.v_scale = c.v_scale;
-  v.k_sp = c.k_stride_p;
-  v.k_sh = c.k_stride_h;
-  v.k_ss = c.k_stride_s;
-  v.v_sp = c.v_stride_p;
-  v.v_sh = c.v_stride_h;
-  v.v_ss = c.v_stride_s;
+  v.k_sp = static_cast<unsigned>(c.k_stride_p);
+  v.k_sh = static_cast<unsigned>(c.k_stride_h);
+  v.k_ss = static_cast<unsigned>(c.k_stride_s);
+  v.v_sp = static_cast<unsigned>(c.v_stride_p);
+  v.v_sh = static_cast<unsigned>(c.v_stride_h);
+  v.v_ss = static_cast<unsigned>(c.v_stride_s);
   v.table = c.page_table;
   v.lens = c.seq_lens;
   v.starts = c.starts;
@@ -75,6 +79,9 @@ inline KvView kv_view(const hb_kv_cache& c, const DeviceState* st) {
 }
 
 #ifdef __CUDACC__
+__device__ __forceinline__ long long kv_offset(int n, unsigned stride) {  // n >= 0: one multiplication
+  return static_cast<long long>(static_cast<unsigned long long>(static_cast<unsigned>(n)) * stride);
+}
 struct KvSeq {
   int start, n;  // its rows of the call
   int len;       // its tokens, those rows included
