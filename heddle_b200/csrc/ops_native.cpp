@@ -42,6 +42,9 @@ struct Lib {
   decltype(&hb_rms_rowstat) rms_rowstat;
   decltype(&hb_row_softmax) row_softmax;
   decltype(&hb_rowwise_program) rowwise_program;
+  decltype(&hb_kv_append) kv_append;
+  decltype(&hb_fa_paged_workspace) fa_paged_workspace;
+  decltype(&hb_fa_paged) fa_paged;
 } lib;
 PyObject* g_check = nullptr;    // _lib.check: raises for a status
 PyObject* g_ew_ops = nullptr;   // _lib.EW_OPS, _lib.EW_SRCS
@@ -370,6 +373,172 @@ PyObject* h2o_score(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int rc = unlocked([&] { return lib.h2o_score(&a); });
   if (rc != HB_OK) return raise_status(rc);
   return THPVariable_Wrap(std::move(score));
+  END_HANDLE_TH_ERRORS
+}
+
+// The cache of a call whose rows are x [T, heads, D]; false where the general path has something to convert or refuse.  pages: the
+// fields of ops.KvPages.
+bool kv_cache(PyObject* pages, PyObject* table, PyObject* lens, PyObject* starts, const at::Tensor& x, int dev, hb_kv_cache& c) {
+  if (!PyTuple_Check(pages) || PyTuple_GET_SIZE(pages) != 5) return false;
+  const at::Tensor* t[4];
+  for (int i = 0; i < 4; ++i)
+    if ((t[i] = plain(PyTuple_GET_ITEM(pages, i), dev)) == nullptr) return false;
+  const at::Tensor &k = *t[0], &v = *t[1];
+  const int layout = layout_of(PyTuple_GET_ITEM(pages, 4));
+  const at::Tensor *pt = plain(table, dev), *sl = plain(lens, dev), *st = starts == Py_None ? nullptr : plain(starts, dev);
+  if (layout < 0 || pt == nullptr || sl == nullptr || (starts != Py_None && st == nullptr)) return false;
+  if (k.dim() != 4 || v.sizes() != k.sizes() || k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn ||
+      k.stride(3) != 1 || v.stride(3) != 1 || x.dim() != 3 || x.size(2) != k.size(3))
+    return false;
+  const int h = layout == 0 ? 1 : 2, s = layout == 0 ? 2 : 1;
+  const int64_t B = pt->dim() == 2 ? pt->size(0) : -1;
+  for (int i = 2; i < 4; ++i)
+    if (t[i]->dim() != 2 || t[i]->size(0) != k.size(0) || t[i]->size(1) != k.size(h) || !contiguous_fp32(*t[i], k.size(0) * k.size(h))) return false;
+  if (B < 0 || pt->scalar_type() != at::kInt || (pt->size(1) > 1 && pt->stride(1) != 1) || sl->scalar_type() != at::kInt || sl->dim() != 1 ||
+      sl->size(0) != B || !sl->is_contiguous())
+    return false;
+  if (st != nullptr && (st->scalar_type() != at::kInt || st->dim() != 1 || st->size(0) != B + 1 || !st->is_contiguous())) return false;
+  for (int64_t n : {k.size(0), k.size(1), k.size(2), k.size(3), B, pt->size(1), x.size(0), x.size(1)})
+    if (!fits_int(n)) return false;
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.k_scale = static_cast<float*>(t[2]->data_ptr());
+  c.v_scale = static_cast<float*>(t[3]->data_ptr());
+  c.k_stride_p = k.stride(0);
+  c.k_stride_h = k.stride(h);
+  c.k_stride_s = k.stride(s);
+  c.v_stride_p = v.stride(0);
+  c.v_stride_h = v.stride(h);
+  c.v_stride_s = v.stride(s);
+  c.num_pages = static_cast<int32_t>(k.size(0));
+  c.page_size = static_cast<int32_t>(k.size(s));
+  c.Hkv = static_cast<int32_t>(k.size(h));
+  c.D = static_cast<int32_t>(k.size(3));
+  c.page_table = static_cast<const int32_t*>(pt->data_ptr());
+  c.seq_lens = static_cast<const int32_t*>(sl->data_ptr());
+  c.starts = st != nullptr ? static_cast<const int32_t*>(st->data_ptr()) : nullptr;
+  c.table_stride = pt->stride(0);
+  c.max_pages = static_cast<int32_t>(pt->size(1));
+  c.B = static_cast<int32_t>(B);
+  c.T = static_cast<int32_t>(x.size(0));
+  return true;
+}
+// [tokens, heads, D] that the kernels read as it lies
+bool rows16(const at::Tensor& t) { return t.dim() == 3 && t.stride(2) == 1 && ((t.stride(0) | t.stride(1)) & 7) == 0 && aligned16(t); }
+
+// kv_append(k, v, pages, page_table, seq_lens, starts, rope, q)
+PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !plain_context()) return general();
+  int dev;
+  const at::Tensor* k = plain_first(args[0], dev);
+  if (k == nullptr) return general();
+  const at::Tensor *v = plain(args[1], dev), *q = args[7] == Py_None ? nullptr : plain(args[7], dev);
+  const int dtype = dtype16(*k);
+  hb_kv_append_args a;
+  std::memset(&a, 0, sizeof(a));
+  if (v == nullptr || (args[7] != Py_None && q == nullptr) || dtype < 0 || v->scalar_type() != k->scalar_type() || !rows16(*k) || !rows16(*v) ||
+      v->sizes() != k->sizes() || !kv_cache(args[2], args[3], args[4], args[5], *k, dev, a.cache) || k->size(1) != a.cache.Hkv)
+    return general();
+  if (args[6] != Py_None) {
+    if (!PyTuple_CheckExact(args[6]) || PyTuple_GET_SIZE(args[6]) != 2) return general();
+    const at::Tensor *cos = plain(PyTuple_GET_ITEM(args[6], 0), dev), *sin = plain(PyTuple_GET_ITEM(args[6], 1), dev);
+    if (cos == nullptr || sin == nullptr || cos->dim() != 2 || cos->size(1) * 2 != a.cache.D || !contiguous_fp32(*cos, cos->numel()) ||
+        sin->sizes() != cos->sizes() || !contiguous_fp32(*sin, cos->numel()) || !aligned16(*cos) || !aligned16(*sin) || !fits_int(cos->size(0)))
+      return general();
+    a.rope_cos = static_cast<const float*>(cos->data_ptr());
+    a.rope_sin = static_cast<const float*>(sin->data_ptr());
+    a.rope_len = static_cast<int32_t>(cos->size(0));
+  }
+  at::Tensor out;
+  if (q != nullptr) {
+    if (q->scalar_type() != k->scalar_type() || !rows16(*q) || q->size(0) != k->size(0) || q->size(2) != k->size(2) || !fits_int(q->size(1))) return general();
+    out = empty_like_options(*q, q->sizes(), q->scalar_type());
+    a.q = q->data_ptr();
+    a.q_out = out.data_ptr();
+    a.Hq = static_cast<int32_t>(q->size(1));
+    a.q_stride_t = q->stride(0);
+    a.q_stride_h = q->stride(1);
+    a.qo_stride_t = q->size(1) * q->size(2);
+    a.qo_stride_h = q->size(2);
+  }
+  a.k = k->data_ptr();
+  a.v = v->data_ptr();
+  a.k_stride_t = k->stride(0);
+  a.k_stride_h = k->stride(1);
+  a.v_stride_t = v->stride(0);
+  a.v_stride_h = v->stride(1);
+  a.dtype = dtype;
+  a.stream = stream_of(dev);
+  const int rc = unlocked([&] { return lib.kv_append(&a); });
+  if (rc != HB_OK) return raise_status(rc);
+  if (q == nullptr) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// fa_paged(q, pages, page_table, seq_lens, starts, max_tokens, causal, softmax_scale, return_lse, out)
+PyObject* fa_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || !plain_context()) return general();
+  int dev;
+  const at::Tensor* q = plain_first(args[0], dev);
+  if (q == nullptr) return general();
+  const int dtype = dtype16(*q);
+  hb_fa_paged_args a;
+  std::memset(&a, 0, sizeof(a));
+  int64_t most = 0;
+  double scale;
+  if (dtype < 0 || q->dim() != 3 || !softmax_scale(args[7], q->size(2), scale)) return general();
+  const int causal = PyObject_IsTrue(args[6]), want_lse = PyObject_IsTrue(args[8]);
+  if (causal < 0 || want_lse < 0) return nullptr;
+  // behind the last line that may run other people's code (__float__, __bool__): pointers are read now
+  if (!rows16(*q) || !kv_cache(args[1], args[2], args[3], args[4], *q, dev, a.cache) ||
+      (args[5] != Py_None && (!integer(args[5], most) || !fits_int(most))))
+    return general();
+  at::Tensor o;
+  if (args[9] != Py_None) {
+    const at::Tensor* given = plain(args[9], dev);
+    if (given == nullptr || given->sizes() != q->sizes() || given->scalar_type() != q->scalar_type() || given->stride(2) != 1) return general();
+    o = *given;
+  } else {
+    o = empty_like_options(*q, q->sizes(), q->scalar_type());
+  }
+  at::Tensor lse;
+  if (want_lse) lse = empty_like_options(*q, {q->size(0), q->size(1)}, at::kFloat);
+  a.q = q->data_ptr();
+  a.o = o.data_ptr();
+  a.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  a.q_stride_t = q->stride(0);
+  a.q_stride_h = q->stride(1);
+  a.o_stride_t = o.stride(0);
+  a.o_stride_h = o.stride(1);
+  a.Hq = static_cast<int32_t>(q->size(1));
+  a.max_tokens = static_cast<int32_t>(most);
+  a.causal = causal;
+  a.softmax_scale = static_cast<float>(scale);
+  a.dtype = dtype;
+  a.stream = stream_of(dev);
+  uint64_t need = 0;
+  int rc = lib.fa_paged_workspace(&a, &need);
+  if (rc != HB_OK) return raise_status(rc);
+  at::Tensor ws;
+  if (need > 0) ws = empty_like_options(*q, {static_cast<int64_t>(need)}, at::kByte);
+  rc = unlocked([&] { return lib.fa_paged(&a, need > 0 ? ws.data_ptr() : nullptr, need); });
+  if (rc != HB_OK) return raise_status(rc);
+  PyObject* result;
+  if (args[9] != Py_None) {
+    result = args[9];
+    Py_INCREF(result);
+  } else {
+    result = THPVariable_Wrap(std::move(o));
+  }
+  if (!want_lse || result == nullptr) return result;
+  PyObject* l = THPVariable_Wrap(std::move(lse));
+  PyObject* pair = l != nullptr ? PyTuple_Pack(2, result, l) : nullptr;
+  Py_DECREF(result);
+  Py_XDECREF(l);
+  return pair;
   END_HANDLE_TH_ERRORS
 }
 
@@ -710,6 +879,9 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HB_BIND(rms_rowstat)
   HB_BIND(row_softmax)
   HB_BIND(rowwise_program)
+  HB_BIND(kv_append)
+  HB_BIND(fa_paged_workspace)
+  HB_BIND(fa_paged)
 #undef HB_BIND
   for (int i = 1; i < 4; ++i) Py_INCREF(args[i]);
   g_check = args[1];
@@ -721,7 +893,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define HB_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HB_METHOD(bind),        HB_METHOD(fa_fwd),      HB_METHOD(fa_bwd),      HB_METHOD(h2o_score),
                          HB_METHOD(gemm_epilogue), HB_METHOD(bmm),       HB_METHOD(rms_rowstat), HB_METHOD(row_softmax),
-                         HB_METHOD(rowwise_program), HB_METHOD(tensors_state), {nullptr, nullptr, 0, nullptr}};
+                         HB_METHOD(rowwise_program), HB_METHOD(kv_append),   HB_METHOD(fa_paged),    HB_METHOD(tensors_state), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Host path of the tensor-level calls (ops.py).", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

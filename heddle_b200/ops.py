@@ -742,7 +742,7 @@ def _kv_cache(who: str, pages: KvPages, page_table, seq_lens, starts, x) -> "_li
 def _rows_16(t: torch.Tensor) -> torch.Tensor:
     """[tokens, heads, D] whose rows the library can read: head_dim contiguous, every row 16-byte aligned."""
     s = t.stride()
-    return t if s[2] == 1 and not (s[0] | s[1]) % 8 and t.data_ptr() % 16 == 0 else t.contiguous()
+    return t if s[2] == 1 and not (s[0] | s[1]) % 8 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, pages: KvPages, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
@@ -760,6 +760,10 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, pages: KvPages, page_table: torc
     A page whose first place is written starts anew; in a page that holds earlier tokens of its sequence the scale grows where the
     new ones need it, and the earlier codes are rounded to it.  A token with an infinity or NaN in a head's key or value becomes a
     NaN key and a zero value there.  Two sequences may share pages that neither appends to."""
+    if _lib.native is not None:
+        r = _lib.native.kv_append(k, v, pages, page_table, seq_lens, starts, rope, q)
+        if r is not NotImplemented:
+            return r
     _require_cuda(k, v, q)
     if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
         raise TypeError(f"kv_append takes bf16 or fp16 rows of one dtype, got {k.dtype}, {v.dtype}" + (f", {q.dtype}" if q is not None else ""))
@@ -805,6 +809,10 @@ def fa_paged(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, seq_lens
     those up to its own position.  ``max_tokens``: the most rows a sequence has, where ``starts`` is given (a hint that chooses
     kernels).  Returns O [T, Hq, D] in q's dtype and, if requested, the natural-log LSE fp32 [T, Hq]; rows without a
     visible key are 0 and -inf.  Rows of no sequence are left as they are in ``out`` (and are whatever new memory holds otherwise)."""
+    if _lib.native is not None:
+        r = _lib.native.fa_paged(q, pages, page_table, seq_lens, starts, max_tokens, causal, softmax_scale, return_lse, out)
+        if r is not NotImplemented:
+            return r
     _require_cuda(q, out)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"fa_paged takes bf16 or fp16 queries, got {q.dtype}")
