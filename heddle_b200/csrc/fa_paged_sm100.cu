@@ -1,5 +1,5 @@
 // hb_fa_paged: checks, the workspace and the launches of the paged attention (fa_paged_sm100.cuh).
-#include "fa_paged_sm100.cuh"
+#include "fa_paged_tiles_sm100.cuh"
 
 #include <algorithm>
 #include <climits>
@@ -46,7 +46,14 @@ static int paged_blocks(const hb_fa_paged_args* a, int sm_count) {
                                        : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
 }
 
+// Which kernels a call takes.  The tiles kernel has the sequences of more than kPagedRowLimit query rows a KV head, the rows kernel the
+// others; where the call says that there are none of the former (or all are), the other one is not launched.
+constexpr int kPagedRowLimit = 64;
+static bool paged_tiles(const hb_fa_paged_args* a) { return paged_most_rows(a) > kPagedRowLimit; }
+static bool paged_rows(const hb_fa_paged_args* a) { return a->cache.starts != nullptr || !paged_tiles(a); }
+
 static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
+  if (!paged_rows(a)) return 0;
   const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
   return 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
 }
@@ -83,6 +90,38 @@ static int launch_rows_of(const FaPagedParams& p, int D, int rows, int blocks, c
   return rows == 8 ? launch_rows<T, 64, 8>(p, blocks, stream) : launch_rows<T, 64, 16>(p, blocks, stream);
 }
 
+template <typename T, int D>
+static int launch_tiles(const FaPagedTilesParams& p, unsigned grid, int smem_optin, cudaStream_t stream) {
+  using Smem = FaPagedTilesSmem<D>;
+  if ((int)sizeof(Smem) > smem_optin)
+    return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: kernel needs %d bytes of shared memory, device offers %d", (int)sizeof(Smem), smem_optin);
+  auto kernel = fa_paged_tiles_kernel<T, D>;
+  static bool configured[64] = {};
+  int dev = 0;
+  HB_CUDA_CHECK(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(g_paged_mutex);
+    if (!configured[dev & 63]) {
+      HB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)));
+      configured[dev & 63] = true;
+    }
+  }
+  HB_CUDA_CHECK(launch_dependent(kernel, grid, kPagedTilesThreads, sizeof(Smem), stream, 0, p));
+  return HB_OK;
+}
+template <typename T>
+static int launch_tiles_of(const FaPagedTilesParams& p, int D, unsigned grid, int smem_optin, cudaStream_t stream) {
+  return D == 128 ? launch_tiles<T, 128>(p, grid, smem_optin, stream) : launch_tiles<T, 64>(p, grid, smem_optin, stream);
+}
+
+// Blocks of the tiles kernel: exactly the items, or where the device knows only, as many as so many rows can be.
+static int64_t paged_tiles_grid(const hb_fa_paged_args* a) {
+  const hb_kv_cache& c = a->cache;
+  const int64_t group = a->Hq / c.Hkv, rows = group * c.T;
+  if (c.starts == nullptr) return static_cast<int64_t>(c.B) * c.Hkv * ((rows / c.B + kPagedBlockRows - 1) / kPagedBlockRows);
+  return c.Hkv * (rows / kPagedBlockRows + std::min<int64_t>(c.B, rows / (kPagedRowLimit + 1)));
+}
+
 }  // namespace hb
 
 extern "C" int hb_fa_paged_workspace(const hb_fa_paged_args* a, uint64_t* bytes) {
@@ -110,32 +149,49 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
   rc = get_device_state(&st);
   if (rc != HB_OK) return rc;
   const uint64_t need = paged_workspace(a, st->sm_count);
-  if (workspace == nullptr || bytes < need)
+  if (need > 0 && (workspace == nullptr || bytes < need))
     return set_error(HB_ERR_BAD_ARG, "hb_fa_paged: needs a workspace of %llu bytes, got %llu", (unsigned long long)need,
                      (unsigned long long)(workspace == nullptr ? 0 : bytes));
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return set_error(HB_ERR_ALIGN, "hb_fa_paged: the workspace must be 16-byte aligned");
   const hb_kv_cache& c = a->cache;
+  const float scale = a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c.D);
+  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+  auto fill = [&](auto& p) {
+    p.c = kv_view(c, st);
+    p.q = a->q;
+    p.o = a->o;
+    p.lse = a->lse;
+    p.q_st = a->q_stride_t;
+    p.q_sh = a->q_stride_h;
+    p.o_st = a->o_stride_t;
+    p.o_sh = a->o_stride_h;
+    p.Hq = a->Hq;
+    p.group = a->Hq / c.Hkv;
+    p.causal = a->causal ? 1 : 0;
+    p.by_group = make_fast_div(p.group);
+    p.scale_log2 = scale * 1.4426950408889634f;
+  };
+  if (paged_tiles(a)) {
+    const int64_t grid = paged_tiles_grid(a);
+    if (grid > 0x7fffffffll) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
+    FaPagedTilesParams p;
+    fill(p);
+    p.row_limit = kPagedRowLimit;
+    p.status = st->status_word;
+    if (grid > 0) {
+      rc = a->dtype == HB_BF16 ? launch_tiles_of<__nv_bfloat16>(p, c.D, static_cast<unsigned>(grid), st->smem_optin, stream)
+                               : launch_tiles_of<__half>(p, c.D, static_cast<unsigned>(grid), st->smem_optin, stream);
+      if (rc != HB_OK) return rc;
+    }
+  }
+  if (!paged_rows(a)) return HB_OK;
   const int rows = paged_tile_rows(a), blocks = paged_blocks(a, st->sm_count);
   FaPagedParams p;
-  p.c = kv_view(c, st);
-  p.q = a->q;
-  p.o = a->o;
-  p.lse = a->lse;
-  p.q_st = a->q_stride_t;
-  p.q_sh = a->q_stride_h;
-  p.o_st = a->o_stride_t;
-  p.o_sh = a->o_stride_h;
-  p.Hq = a->Hq;
-  p.group = a->Hq / c.Hkv;
-  p.causal = a->causal ? 1 : 0;
-  p.row_limit = INT_MAX;
-  p.by_group = make_fast_div(p.group);
-  const float scale = a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)c.D);
-  p.scale_log2 = scale * 1.4426950408889634f;
+  fill(p);
+  p.row_limit = paged_tiles(a) ? kPagedRowLimit : INT_MAX;
   p.heads = static_cast<PagedHead*>(workspace);
   p.part_o = reinterpret_cast<float*>(p.heads + blocks);
   p.part_lse = p.part_o + 2ll * blocks * rows * c.D;
-  cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   return a->dtype == HB_BF16 ? launch_rows_of<__nv_bfloat16>(p, c.D, rows, blocks, stream)
                              : launch_rows_of<__half>(p, c.D, rows, blocks, stream);
 }

@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
   constexpr int kN = kRows / 8;   // tiles of query rows
   constexpr float kGrowth = 7.f, kPUnit = 256.f;
-  extern __shared__ __align__(128) uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const KvView& kv = p.c;

@@ -1,0 +1,566 @@
+// Attention of many query rows (prompts, chunks of them) over the paged 8-bit cache (hb_fa_paged), sm_100a.
+//
+// Bound by the tensor cores and the exponentials, as fa_fwd: 256 query rows of one (sequence, KV head) a block, row = token * group +
+// head, against key tiles of 128, S and O in TMEM, P over S.  What differs is what feeds it:
+//   - four producer warps fetch the codes of a tile's pages (whatever their order), convert them to fp16 and store them as the
+//     operands that tcgen05.mma reads (128-byte swizzle; keys K-major, values MN-major), each tile once for 256 rows.  Two
+//     e4m3 products of a query's and a weight's parts would need no conversion, and twice the products and a split of every weight;
+//   - the scales of a tile's pages are taken relative to the tile's largest, powers of two that fp16 holds beside the code; where all
+//     are alike, nearly always, nothing is multiplied.  The largest goes into the factor of the scores and the unit of P';
+//   - queries are scaled into fp16 by a power of two for each row, by the thread that owns the row.
+// A row's maximum is adopted when it grew by more than 2^7, and O's unit when a tile has a larger value scale: P' = 256 P
+// (scale / unit).  O is rescaled by the row's own thread, as in fa_split.
+#pragma once
+
+#include "fa_fwd_sm100.cuh"
+#include "fa_paged_sm100.cuh"
+
+namespace hb {
+
+constexpr int kPagedTilesThreads = 512;  // 8 softmax warps, the MMA warp (and three idle ones), 4 producers
+constexpr int kPagedBlockRows = 2 * kTileM;
+enum FaPagedRole : uint32_t { kRolePagedSoftmax = 10, kRolePagedMma = 11, kRolePagedProducer = 12, kRolePagedDrain = 13 };
+
+struct FaPagedTilesParams {
+  KvView c;
+  const void* q;
+  void* o;
+  float* lse;
+  long long q_st, q_sh, o_st, o_sh;
+  int Hq, group, causal;
+  int row_limit;  // sequences with no more query rows a KV head are the rows kernel's
+  FastDiv by_group;
+  float scale_log2;
+  uint32_t* status;
+};
+
+template <int D>
+struct FaPagedTilesSmem {
+  static constexpr int kTileBytes = kTileN * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  alignas(1024) uint8_t q[2][kTileBytes];
+  alignas(1024) uint8_t kv[kStages][kTileBytes];
+  static constexpr int kMeta = 8;
+  // K(j + kMeta) takes the ring's place of tile 2 (j + kMeta) - kStages of K(0) V(0) K(1) V(1) ..: where that is V(j) or later, P(j) was
+  // there, and so meta(j) read
+  static_assert(2 * kMeta - kStages >= 1, "a tile's scales are overwritten only when its softmax is done");
+  float4 meta[kMeta];  // of key tile j at j % kMeta: largest key scale, largest value scale, bits of groups of 16 keys that are not there
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t meta_full[kMeta];
+  uint64_t drain;
+  long long sums[kPagedTilesThreads / 32];
+  long long found_at;
+  int found;
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+};
+
+struct PagedItem {
+  KvSeq s;
+  int b, h, row0, rows;  // rows of the sequence in this KV head
+  int n[2];              // key tiles of the two row tiles, 0: no rows
+};
+
+__device__ __forceinline__ int paged_blocks_of(const FaPagedTilesParams& p, const KvSeq& s) {
+  const long long rows = static_cast<long long>(s.n) * p.group;
+  return rows > p.row_limit ? static_cast<int>((rows + kPagedBlockRows - 1) / kPagedBlockRows) : 0;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, FaPagedTilesSmem<D>& s, const AbortCtx& ctx, uint32_t tmem,
+                                                   const PagedItem& it, int i) {
+  using Smem = FaPagedTilesSmem<D>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = threadIdx.x & (kTileM - 1);
+  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t tS = tmem + lane_off + static_cast<uint32_t>(i * kTileN), tO = tmem + lane_off + 256u + static_cast<uint32_t>(i * 128);
+  const int n = i == 0 ? it.n[0] : it.n[1];
+  if (n == 0) return;
+  const int first = it.row0 + kTileM * i, row = first + r;
+  const bool live = row < it.rows;
+  const int tok = live ? fast_div(row, p.by_group) : 0, head = it.h * p.group + (live ? row - tok * p.group : 0);
+  const int limit = !live ? 0 : p.causal ? min(it.s.len, it.s.pos0() + tok + 1) : it.s.len;
+  const int least = p.causal ? min(it.s.len, it.s.pos0() + fast_div(first, p.by_group) + 1) : it.s.len;
+
+  float factor;
+  {  // the row's queries in fp16: 2^up takes the largest element into [2^14, 2^15)
+    const T* src = static_cast<const T*>(p.q) + static_cast<long long>(it.s.start + tok) * p.q_st + head * p.q_sh;
+    uint4 w[D / 8];
+    float top = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < D / 8; ++e) w[e] = live ? *reinterpret_cast<const uint4*>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int e = 0; e < D / 8; ++e) {
+      const uint32_t u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        Pack2<T>::unpack(u[k], a, b);
+        top = max3(top, fabsf(a), fabsf(b));
+        finite = finite && fabsf(a) <= 3.402823466e38f && fabsf(b) <= 3.402823466e38f;
+      }
+    }
+    int up = 0;
+    if (top > 0.f && top <= 3.402823466e38f) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
+    const float mul = __int_as_float((up + 127) << 23);
+    factor = finite ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int e = 0; e < D / 8; ++e) {
+      uint32_t u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        Pack2<T>::unpack(u[k], a, b);
+        u[k] = Pack2<__half>::pack(a * mul, b * mul);
+      }
+      *reinterpret_cast<uint4*>(s.q[i] + (e >> 3) * (kTileM * 128) + r * 128 + ((e & 7) ^ (r & 7)) * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.q_full[i]);
+  }
+
+  float m = -INFINITY, l = 0.f, v_unit = 0.f;
+  for (int j = 0; j < n; ++j) {
+    if (!mbar_wait_warp(&s.s_full[i], j & 1, ctx, kRolePagedSoftmax)) return;
+    tc_fence_after();
+    uint32_t v[kTileN];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, &v[c * 32]);
+    if (!mbar_wait_warp(&s.meta_full[j % Smem::kMeta], (j / Smem::kMeta) & 1, ctx, kRolePagedSoftmax)) return;
+    const float4 meta = s.meta[j % Smem::kMeta];
+    const uint32_t gone = __float_as_uint(meta.z);
+    tmem_wait_ld();
+
+    const int col0 = j * kTileN;
+    if (col0 + kTileN > least || gone != 0u) {
+      const int lim = limit - 1 - col0;
+#pragma unroll
+      for (int c = 0; c < kTileN; ++c) v[c] = (c <= lim && !((gone >> (c >> 4)) & 1u)) ? v[c] : 0xff800000u;  // -inf
+    }
+    float mx[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(v[c]);
+#pragma unroll
+    for (int c = 4; c < kTileN; c += 8) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c + 4 < kTileN) mx[e] = max3(mx[e], __uint_as_float(v[c + e]), __uint_as_float(v[c + 4 + e]));
+        else mx[e] = fmaxf(mx[e], __uint_as_float(v[c + e]));
+      }
+    }
+    float f = factor * meta.x;
+    f = f == 0.f ? 1.17549435e-38f : f;  // -inf has to stay it
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+    const bool adopt = live && top > m + 7.f;  // padding rows never ask for a rescale
+    float alpha = adopt ? fast_exp2(m - top) : 1.f;
+    m = adopt ? top : m;
+    l *= alpha;
+    // P' = 2^(x f - m + e) with 2^e = 256 (the tile's value scale / the unit)
+    int e = 8;
+    if (meta.y > v_unit) {
+      alpha *= v_unit / meta.y;  // 0 at first
+      v_unit = meta.y;
+    } else if (meta.y > 0.f) {
+      e = max(8 + (__float_as_int(meta.y) >> 23) - (__float_as_int(v_unit) >> 23), -64);
+    }
+    const float off = static_cast<float>(e) - (m == -INFINITY ? 0.f : m);
+
+    const uint64_t f2 = pack_f32x2(f, f), off2 = pack_f32x2(off, off);
+    uint64_t sa = pack_f32x2(0.f, 0.f), sb = sa;
+#pragma unroll
+    for (int q = 0; q < kTileN / 32; ++q) {
+      uint32_t pk[16];
+#pragma unroll
+      for (int k = 0; k < 32; k += 4) {
+        const int c = q * 32 + k;
+        const uint64_t x0 = fma_f32x2(pack_f32x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), f2, off2);
+        const uint64_t x1 = fma_f32x2(pack_f32x2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), f2, off2);
+        float a0, a1, b0, b1;
+        unpack_f32x2(x0, a0, a1);
+        unpack_f32x2(x1, b0, b1);
+        a0 = fast_exp2(a0);
+        a1 = fast_exp2(a1);
+        b0 = fast_exp2(b0);
+        b1 = fast_exp2(b1);
+        sa = add_f32x2(sa, pack_f32x2(a0, a1));
+        sb = add_f32x2(sb, pack_f32x2(b0, b1));
+        pk[k / 2] = Pack2<__half>::pack(a0, a1);
+        pk[k / 2 + 1] = Pack2<__half>::pack(b0, b1);
+      }
+      tmem_st16(tS + q * 16, pk);
+    }
+    float sum0, sum1, sum2, sum3;
+    unpack_f32x2(sa, sum0, sum1);
+    unpack_f32x2(sb, sum2, sum3);
+    l = fmaf((sum0 + sum1) + (sum2 + sum3), __int_as_float((127 - e) << 23), l);
+    // S(j) was committed behind P V(j - 1), so that product is complete, and P V(j) is only issued after this warp's arrival
+    if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + c * 32, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+        tmem_st32(tO + c * 32, o);
+      }
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.p_full[i]);
+  }
+
+  if (!mbar_wait_warp(&s.o_full[i], 0, ctx, kRolePagedSoftmax)) return;
+  tc_fence_after();
+  const float inv = l != 0.f ? v_unit * (1.f / 256.f) / l : 0.f;  // a row without keys is 0, one with a NaN is NaN
+  T* dst = static_cast<T*>(p.o) + static_cast<long long>(it.s.start + tok) * p.o_st + head * p.o_sh;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    __syncwarp();
+    tmem_ld32(tO + c * 32, o);
+    tmem_wait_ld();
+    uint4 w[4];
+    pack_row32<T>(o, inv, w);
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(dst + c * 32 + k * 8) = w[k];
+    }
+  }
+  if (live && p.lse != nullptr)
+    p.lse[static_cast<long long>(it.s.start + tok) * p.Hq + head] =
+        (l != 0.f ? (m == -INFINITY ? 0.f : m) + fast_log2(l) : -INFINITY) * 0.6931471805599453f;
+}
+
+template <int D>
+__device__ __forceinline__ void paged_mma_role(FaPagedTilesSmem<D>& s, const AbortCtx& ctx, uint32_t tmem, const PagedItem& it) {
+  using Smem = FaPagedTilesSmem<D>;
+  constexpr uint32_t kFmt = Pack2<__half>::kFormat;
+  constexpr uint32_t idesc_qk = make_idesc(kFmt, kTileM, kTileN, 0, 0);
+  constexpr uint32_t idesc_pv = make_idesc(kFmt, kTileM, D, 0, 1);
+  constexpr uint32_t kSub = kTileM * 128u >> 4;                   // next 64 columns of head_dim
+  constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // see fa_mma_role
+  constexpr uint32_t kLboK = (16u >> 4) << 16, kLboV = kSub << 16;
+  constexpr uint32_t kTile16 = Smem::kTileBytes >> 4;
+  auto desc = [](uint32_t lo) -> uint64_t { return (static_cast<uint64_t>(kDescHi) << 32) | lo; };
+  const uint32_t q_lo = (smem_u32(s.q[0]) >> 4) | kLboK, kv_lo = smem_u32(s.kv[0]) >> 4;
+  const bool leader = elect_one();
+  auto commit = [&](uint64_t* bar) {
+    if (leader) umma_commit(bar);
+  };
+  auto issue_qk = [&](int i, uint32_t slot) {
+    const uint32_t qa = q_lo + static_cast<uint32_t>(i) * kTile16, ka = (kv_lo + slot * kTile16) | kLboK;
+    if (leader) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = static_cast<uint32_t>(kk >> 2) * kSub + static_cast<uint32_t>(kk & 3) * 2u;
+        umma_ss_f16(tmem + static_cast<uint32_t>(i * kTileN), desc(qa + off), desc(ka + off), idesc_qk, kk > 0 ? 1u : 0u);
+      }
+    }
+  };
+  auto issue_pv = [&](int i, uint32_t slot, uint32_t accumulate) {
+    const uint32_t va = (kv_lo + slot * kTile16) | kLboV, tS = tmem + static_cast<uint32_t>(i * kTileN);
+    if (leader) {
+#pragma unroll
+      for (int kk = 0; kk < kTileN / 16; ++kk)
+        umma_ts_f16(tmem + 256u + static_cast<uint32_t>(i * 128), tS + static_cast<uint32_t>(kk * 8), desc(va + static_cast<uint32_t>(kk) * (16u * 128u >> 4)),
+                    idesc_pv, kk > 0 ? 1u : accumulate);
+    }
+  };
+  uint32_t slot = 0, phase = 0;
+  auto advance = [&]() {
+    if (++slot == Smem::kStages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  };
+  const int nmax = max(it.n[0], it.n[1]);
+  uint32_t slot_k = slot;
+  if (!mbar_wait_warp(&s.kv_full[slot], phase, ctx, kRolePagedMma)) return;
+  advance();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if ((i == 0 ? it.n[0] : it.n[1]) == 0) continue;
+    if (!mbar_wait_warp(&s.q_full[i], 0, ctx, kRolePagedMma)) return;
+    tc_fence_after();
+    issue_qk(i, slot_k);
+    commit(&s.s_full[i]);
+  }
+  commit(&s.kv_empty[slot_k]);
+  for (int j = 0; j < nmax; ++j) {
+    const uint32_t slot_v = slot;
+    if (!mbar_wait_warp(&s.kv_full[slot], phase, ctx, kRolePagedMma)) return;
+    advance();
+    const bool has_next = j + 1 < nmax;
+    bool k_ready = false;
+    slot_k = slot;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const int ni = i == 0 ? it.n[0] : it.n[1];
+      if (j < ni) {
+        if (!mbar_wait_warp(&s.p_full[i], j & 1, ctx, kRolePagedMma)) return;
+        tc_fence_after();
+        issue_pv(i, slot_v, j > 0 ? 1u : 0u);
+        if (j == ni - 1) commit(&s.o_full[i]);
+      }
+      if (j + 1 < ni) {
+        if (!k_ready) {
+          if (!mbar_wait_warp(&s.kv_full[slot], phase, ctx, kRolePagedMma)) return;
+          tc_fence_after();
+          k_ready = true;
+        }
+        issue_qk(i, slot_k);
+        commit(&s.s_full[i]);
+      }
+    }
+    commit(&s.kv_empty[slot_v]);
+    if (has_next) {
+      commit(&s.kv_empty[slot_k]);
+      advance();
+    }
+  }
+}
+
+// Producer warp pw has rows 32 pw .. + 31 of every tile.  A quarter of a warp reads 64 bytes of two rows next to each other: their
+// fp16 chunks then lie in all eight places of a 128-byte line.
+template <int D>
+__device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p, FaPagedTilesSmem<D>& s, const AbortCtx& ctx,
+                                                    const PagedItem& it, int pw) {
+  using Smem = FaPagedTilesSmem<D>;
+  constexpr int kRowsAtOnce = 512 / D, kCopies = 32 / kRowsAtOnce;
+  const KvView& kv = p.c;
+  const int lane = threadIdx.x & 31, quarter = lane >> 3, l8 = lane & 7;
+  const int rr = D == 128 ? 2 * (quarter >> 1) + (l8 >> 2) : 2 * quarter + (l8 >> 2);
+  const int ch = D == 128 ? 4 * (quarter & 1) + (l8 & 3) : (l8 & 3);  // 16 codes
+  uint32_t dst[2][2];  // of the lane's two fp16 chunks; rows eight apart (one or two copies) have the same swizzle
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int row = 32 * pw + (k * kRowsAtOnce) % 8 + rr;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) dst[k][x] = (ch >> 2) * (kTileN * 128) + row * 128 + ((2 * (ch & 3) + x) ^ (row & 7)) * 16;
+  }
+  const int nmax = max(it.n[0], it.n[1]), len = it.s.len;
+
+  // of key tile j, in lane g < 8: page and scales of keys 16 g .. + 15 (-1 and 0: none of the cache's, or behind the sequence)
+  auto page_of = [&](int j) -> int {
+    const int tok = j * kTileN + 16 * l8;
+    return j < nmax && tok < len ? kv_page(kv, it.b, tok >> kv.page_shift) : -1;
+  };
+  auto scale_of = [&](const float* scales, int page) -> float {
+    return page >= 0 ? scales[static_cast<long long>(page) * kv.Hkv + it.h] : 0.f;
+  };
+  auto fetch = [&](const uint8_t* base, unsigned sp, unsigned ss, int j, int page, uint4 (&w)[kCopies]) {
+    const int tok = j * kTileN + 32 * pw, at = tok & ((1 << kv.page_shift) - 1);
+    const int page0 = __shfl_sync(0xffffffffu, page, 2 * pw), page1 = __shfl_sync(0xffffffffu, page, 2 * pw + 1);
+    const uint8_t* p0 = base + kv_offset(page0, sp) + kv_offset(at + rr, ss) + ch * 16;
+    const uint8_t* p1 = base + kv_offset(page1, sp) + kv_offset((kv.page_shift == 4 ? 0 : at + 16) + rr, ss) + ch * 16;
+    const long long step = kv_offset(kRowsAtOnce, ss);
+#pragma unroll
+    for (int k = 0; k < kCopies; ++k) {
+      const int half = k / (kCopies / 2), k2 = k % (kCopies / 2);
+      const bool real = (half == 0 ? page0 : page1) >= 0 && tok + k * kRowsAtOnce + rr < len;
+      w[k] = real ? *reinterpret_cast<const uint4*>((half == 0 ? p0 : p1) + k2 * step) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  auto store = [&](uint32_t slot, const uint4 (&w)[kCopies], bool alike, __half2 r0, __half2 r1) {
+    const uint32_t tile = smem_u32(s.kv[slot]);
+#pragma unroll
+    for (int k = 0; k < kCopies; ++k) {
+      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      uint32_t h[8];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) codes_f16(u[x], h[2 * x], h[2 * x + 1]);
+      if (!alike) {
+        const __half2 r = k < kCopies / 2 ? r0 : r1;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[x]), r);
+          h[x] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+      }
+      constexpr int kSame = 8 / kRowsAtOnce;  // copies until the swizzle repeats: 2 (D 128), 1 (D 64)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + dst[k % kSame][x] + (k / kSame) * 8 * 128), "r"(h[4 * x]),
+                     "r"(h[4 * x + 1]), "r"(h[4 * x + 2]), "r"(h[4 * x + 3])
+                     : "memory");
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.kv_full[slot]);
+  };
+
+  const uint8_t* k_base = kv.k + kv_offset(it.h, kv.k_sh);
+  const uint8_t* v_base = kv.v + kv_offset(it.h, kv.v_sh);
+  uint32_t slot = 0, phase = 1;  // "empty" barriers start out free
+  auto advance = [&]() {
+    if (++slot == Smem::kStages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  };
+  int page = page_of(0);
+  float ks = scale_of(kv.k_scale, page), vs = scale_of(kv.v_scale, page);
+  uint4 wk[kCopies], wv[kCopies];
+  fetch(k_base, kv.k_sp, kv.k_ss, 0, page, wk);
+  for (int j = 0; j < nmax; ++j) {
+    const int next = page_of(j + 1);
+    fetch(v_base, kv.v_sp, kv.v_ss, j, page, wv);
+    // the tile's largest scales, and this warp's two halves relative to them
+    float k_ref = ks, v_ref = vs;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      k_ref = fmaxf(k_ref, __shfl_xor_sync(0xffffffffu, k_ref, o));
+      v_ref = fmaxf(v_ref, __shfl_xor_sync(0xffffffffu, v_ref, o));
+    }
+    const float k_inv = k_ref > 0.f ? 1.f / k_ref : 0.f, v_inv = v_ref > 0.f ? 1.f / v_ref : 0.f;
+    const bool inside = j * kTileN + 16 * l8 < len;
+    const uint32_t gone = __ballot_sync(0xffffffffu, inside && ks == 0.f) & 0xffu;
+    const bool k_alike = __all_sync(0xffffffffu, ks == 0.f || ks == k_ref), v_alike = __all_sync(0xffffffffu, vs == v_ref || page < 0);
+    const __half2 kr0 = __float2half2_rn(__shfl_sync(0xffffffffu, ks, 2 * pw) * k_inv), kr1 = __float2half2_rn(__shfl_sync(0xffffffffu, ks, 2 * pw + 1) * k_inv);
+    const __half2 vr0 = __float2half2_rn(__shfl_sync(0xffffffffu, vs, 2 * pw) * v_inv), vr1 = __float2half2_rn(__shfl_sync(0xffffffffu, vs, 2 * pw + 1) * v_inv);
+    if (pw == 0 && __any_sync(0xffffffffu, inside && page < 0) && lane == 0) kv_report(kv, HB_CACHE_BAD_PAGE);
+
+    if (!mbar_wait_warp(&s.kv_empty[slot], phase, ctx, kRolePagedProducer)) return;
+    if (pw == 0 && lane == 0) {
+      s.meta[j % Smem::kMeta] = make_float4(k_ref, v_ref, __uint_as_float(gone), 0.f);
+      mbar_arrive(&s.meta_full[j % Smem::kMeta]);
+    }
+    store(slot, wk, k_alike, kr0, kr1);
+    advance();
+    if (j + 1 < nmax) fetch(k_base, kv.k_sp, kv.k_ss, j + 1, next, wk);
+    ks = scale_of(kv.k_scale, next);
+    vs = scale_of(kv.v_scale, next);
+    if (!mbar_wait_warp(&s.kv_empty[slot], phase, ctx, kRolePagedProducer)) return;
+    store(slot, wv, v_alike, vr0, vr1);
+    advance();
+    page = next;
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(const __grid_constant__ FaPagedTilesParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  using Smem = FaPagedTilesSmem<D>;
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  AbortCtx ctx{&s.abort_flag, p.status};
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    s.found = -1;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 4);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.o_full[i], 1);
+    }
+    for (int i = 0; i < Smem::kStages; ++i) {
+      mbar_init(&s.kv_full[i], 4);
+      mbar_init(&s.kv_empty[i], 1);
+    }
+    for (int i = 0; i < Smem::kMeta; ++i) mbar_init(&s.meta_full[i], 1);
+    mbar_init(&s.drain, 1);
+    fence_mbar_init();
+    if ((smem_u32(smem_raw) & 1023u) != 0u) raise_abort(ctx, kStatusSmemMisaligned);
+  }
+  __syncthreads();
+  grid_wait();
+
+  // ---- the block's item: sequences in order, within one the last 256 rows (which see most keys) of every KV head first
+  PagedItem it;
+  {
+    const KvView& kv = p.c;
+    long long before = 0;
+    for (int b0 = 0; b0 < kv.B && before <= blockIdx.x; b0 += kPagedTilesThreads) {
+      const int b = b0 + threadIdx.x;
+      const long long own = b < kv.B ? static_cast<long long>(paged_blocks_of(p, kv_seq(kv, b))) * kv.Hkv : 0;
+      long long upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      if (b0 > 0) __syncthreads();
+      if (lane == 31) s.sums[warp] = upto;
+      __syncthreads();
+      upto += before;
+      for (int w = 0; w < kPagedTilesThreads / 32; ++w) {
+        if (w < warp) upto += s.sums[w];
+        before += s.sums[w];
+      }
+      if (upto > blockIdx.x && upto - own <= blockIdx.x) {
+        s.found = b;
+        s.found_at = upto - own;
+      }
+    }
+    if (blockIdx.x == 0) {
+      for (int b = threadIdx.x; b < kv.B; b += kPagedTilesThreads) {
+        const uint32_t f = kv_seq_faults(kv, b);
+        if (f != 0) kv_report(kv, f);
+      }
+    }
+    __syncthreads();
+    if (s.found < 0) return;  // the grid is cut for the most items that so many rows can be
+    it.b = s.found;
+    it.s = kv_seq(kv, it.b);
+    const int in = static_cast<int>(blockIdx.x - s.found_at), rank = in / kv.Hkv;
+    it.h = in - rank * kv.Hkv;
+    it.rows = it.s.n * p.group;
+    it.row0 = (paged_blocks_of(p, it.s) - 1 - rank) * kPagedBlockRows;
+    const int tiles = max((it.s.len + kTileN - 1) / kTileN, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r0 = it.row0 + kTileM * i;
+      if (r0 >= it.rows) {
+        it.n[i] = 0;
+      } else if (p.causal) {
+        const int last = it.s.pos0() + fast_div(min(r0 + kTileM, it.rows) - 1, p.by_group);  // position of the last row
+        it.n[i] = max(min(tiles, last / kTileN + 1), 1);
+      } else {
+        it.n[i] = tiles;
+      }
+    }
+  }
+
+  if (warp == 8) {
+    tmem_alloc(&s.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = warp_uniform(s.tmem_base);
+  const bool run = s.abort_flag == 0;
+  // 512 threads start with 128 registers each: four warps return 80, four 16, eight grow by 48
+  static_assert(8 * 32 * (176 - 128) <= 4 * 32 * (128 - 48) + 4 * 32 * (128 - 112), "setmaxnreg budget does not balance");
+  if (warp < 8) {
+    reg_inc<176>();
+    if (run) paged_softmax_role<T, D>(p, s, ctx, tmem, it, warp >> 2);
+  } else if (warp < 12) {
+    reg_dec<48>();
+    if (run && warp == 8) {
+      paged_mma_role<D>(s, ctx, tmem, it);
+      __syncwarp();
+      if (s.abort_flag && lane == 0) {
+        umma_commit(&s.drain);  // aborting: let the tensor pipe drain before TMEM is released
+        mbar_wait(&s.drain, 0, ctx, kRolePagedDrain);
+      }
+    }
+  } else {
+    reg_dec<112>();
+    if (run) paged_producer_role<D>(p, s, ctx, it, warp - 12);
+  }
+  __syncwarp();
+  tc_fence_before();
+  grid_launch_dependents();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace hb
