@@ -12,8 +12,14 @@ namespace hb {
 constexpr int kPagedTile = 32;   // keys of a tile: what a warp works through at a time
 constexpr int kPagedWarps = 4;   // of a block; they take the tiles of its run in turn
 
+// What a run pays for an item that it starts or goes on with, in tiles of the list: its queries, the meeting of the warps, the store
+// (about 5000 cycles, and a tile takes a warp 3000).  An item has so many places in front of its tiles; a run that ends among
+// them leaves the item to the next one.
+constexpr int kPagedItemCost = 6;
+
 // Key tiles of an item with `len` keys (an item without keys has a tile all the same: somebody has to write its rows).
 HB_HD int paged_tiles(int len) { return len <= 0 ? 1 : (len + kPagedTile - 1) / kPagedTile; }
+HB_HD int paged_places(int tiles) { return tiles + kPagedItemCost; }
 HB_HD int paged_row_tiles(int n, int group, int rows) {
   return static_cast<int>((static_cast<long long>(n) * group + rows - 1) / rows);
 }
@@ -30,7 +36,11 @@ HB_HD long long paged_begin(long long total, int runs, int w) {  // total < 2^48
   const long long per = paged_div(total, runs);
   return per * w + paged_div((total - per * runs) * w, runs);
 }
-// The run of tile t: the last w with begin(w) = floor(w total / runs) <= t.
-HB_HD int paged_run_of(long long total, int runs, long long t) { return static_cast<int>(((t + 1) * runs - 1) / total); }
+// a / b for any a and b that fit
+HB_HD long long paged_div64(long long a, long long b) {
+  return ((a | b) >> 31) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+// The run of place t: the last w with begin(w) = floor(w total / runs) <= t.
+HB_HD int paged_run_of(long long total, int runs, long long t) { return static_cast<int>(paged_div64((t + 1) * runs - 1, total)); }
 
 }  // namespace hb

@@ -5,6 +5,7 @@
 #include <climits>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 #include "host_common.h"
@@ -40,20 +41,25 @@ static int64_t paged_most_rows(const hb_fa_paged_args* a) {
 }
 static int paged_tile_rows(const hb_fa_paged_args* a) { return paged_most_rows(a) <= 8 ? 8 : kPagedMaxRows; }
 
+// As many blocks as the device holds, and no more than the list can fill: of tiles that the page table has room for.
 static int paged_blocks(const hb_fa_paged_args* a, int sm_count) {
+  const hb_kv_cache& c = a->cache;
   const bool few = paged_tile_rows(a) == 8;
-  return sm_count * (a->cache.D == 128 ? (few ? paged_blocks_per_sm<128, 8> : paged_blocks_per_sm<128, 16>)
-                                       : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
+  const int most = sm_count * (c.D == 128 ? (few ? paged_blocks_per_sm<128, 8> : paged_blocks_per_sm<128, 16>)
+                                          : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
+  const double row_tiles = (double)c.T * (a->Hq / c.Hkv) / paged_tile_rows(a) + c.B;
+  const double runs = row_tiles * c.Hkv * paged_places(paged_tiles(c.max_pages * c.page_size)) / kPagedWarps + 1;
+  return runs < most ? (int)runs : most;
 }
 
 // Which kernels a call takes.  The tiles kernel has the sequences of more than kPagedRowLimit query rows a KV head, the rows kernel the
 // others; where the call says that there are none of the former (or all are), the other one is not launched.
 constexpr int kPagedRowLimit = 64;
-static bool paged_tiles(const hb_fa_paged_args* a) { return paged_most_rows(a) > kPagedRowLimit; }
-static bool paged_rows(const hb_fa_paged_args* a) { return a->cache.starts != nullptr || !paged_tiles(a); }
+static bool paged_takes_tiles(const hb_fa_paged_args* a) { return paged_most_rows(a) > kPagedRowLimit; }
+static bool paged_takes_rows(const hb_fa_paged_args* a) { return a->cache.starts != nullptr || !paged_takes_tiles(a); }
 
 static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
-  if (!paged_rows(a)) return 0;
+  if (!paged_takes_rows(a)) return 0;
   const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
   return 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
 }
@@ -77,7 +83,8 @@ static int launch_rows(const FaPagedParams& p, int blocks, cudaStream_t stream) 
   const long long items = static_cast<long long>(p.c.B) * p.c.Hkv;
   const long long parts = (blocks + items - 1) / items + 1;
   if (parts <= 8) {
-    HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, true>, blocks * kRows / 8, 32 * 8, 0, stream, 0, p, kRows));
+    const int per_block = kPagedCombineWarps;
+    HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, true>, blocks * kRows / per_block, 32 * per_block, 0, stream, 0, p, kRows));
   } else {
     const unsigned warps = static_cast<unsigned>(std::min<long long>(kPagedCombineWarps, (parts + 3) / 4));
     HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, false>, blocks * kRows, 32 * warps, 0, stream, 0, p, kRows));
@@ -171,7 +178,7 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
     p.by_group = make_fast_div(p.group);
     p.scale_log2 = scale * 1.4426950408889634f;
   };
-  if (paged_tiles(a)) {
+  if (paged_takes_tiles(a)) {
     const int64_t grid = paged_tiles_grid(a);
     if (grid > 0x7fffffffll) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
     FaPagedTilesParams p;
@@ -184,11 +191,23 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
       if (rc != HB_OK) return rc;
     }
   }
-  if (!paged_rows(a)) return HB_OK;
+  if (!paged_takes_rows(a)) return HB_OK;
   const int rows = paged_tile_rows(a), blocks = paged_blocks(a, st->sm_count);
   FaPagedParams p;
   fill(p);
-  p.row_limit = paged_tiles(a) ? kPagedRowLimit : INT_MAX;
+  p.row_limit = paged_takes_tiles(a) ? kPagedRowLimit : INT_MAX;
+  p.status = st->status_word;
+  for (const bool keys : {true, false}) {
+    // an axis of one page, head or token may carry any stride
+    const uint64_t dims[4] = {(uint64_t)c.D, (uint64_t)c.page_size, (uint64_t)c.Hkv, (uint64_t)std::max(c.num_pages, 1)};
+    const int64_t given[3] = {keys ? c.k_stride_s : c.v_stride_s, keys ? c.k_stride_h : c.v_stride_h, keys ? c.k_stride_p : c.v_stride_p};
+    uint64_t strides[3];
+    for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (uint64_t)given[i] : (uint64_t)c.D;
+    const uint32_t box[4] = {(uint32_t)c.D, (uint32_t)std::min(c.page_size, kPagedTile), 1, 1};
+    rc = encode_tensor_map(keys ? &p.tm_k : &p.tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box,
+                           c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc != HB_OK) return rc;
+  }
   p.heads = static_cast<PagedHead*>(workspace);
   p.part_o = reinterpret_cast<float*>(p.heads + blocks);
   p.part_lse = p.part_o + 2ll * blocks * rows * c.D;

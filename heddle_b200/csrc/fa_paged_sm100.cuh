@@ -9,8 +9,8 @@
 // product by product (5.9 cycles of an SM for m16n8k32 against 2.0 for the fp16 product of half that depth).  So the codes are A and the
 // few query rows B: S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T, and nothing is padded beyond 8 rows.
 //
-// A warp works through tiles of 32 keys alone, from its own ring in shared memory, filled by 16-byte asynchronous copies, which
-// leave out (as zeros) what lies behind the sequence.  Keys are numbered within a group of eight so that both readings of a tile (keys
+// A warp works through tiles of 32 keys alone, from its own ring in shared memory, filled by TMA copies of a page's tokens (as 16-byte
+// asynchronous copies of each lane a tile's loads took 800 of its 3000 cycles).  Keys are numbered within a group of eight so that both readings of a tile (keys
 // along their rows, values across them) are free of bank conflicts; P goes from S^T's layout into B's by a transposing move,
 // and the pairs of value rows that a lane needs are put together by byte permutations.
 // A row's maximum is adopted when it grew by more than 2^7, as in fa_fwd: P' = 256 P vscale / v_ref stays within fp16.
@@ -27,15 +27,18 @@ namespace hb {
 
 constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedMaxRows = 16;
+constexpr uint32_t kRolePagedRows = 14;
 
-struct PagedHead {  // of an item in parts: where its parts lie (one a run; written by the run that starts the item)
-  int b, h, rt;
-  int last;  // run of its last part, -1: this run starts no item in parts
-  int slot;  // of its first part
-  int pad[3];
+struct alignas(16) PagedHead {  // of an item in parts: where its parts lie (one a run; written by the run that starts the item)
+  int last;         // run of its last part, -1: this run starts no item in parts
+  int slot;         // of its first part
+  int h, row0;      // KV head, first row of the row tile
+  int start, rows;  // of the sequence: its first row of the call, its query rows in a KV head
+  int pad[2];
 };
 
-struct FaPagedParams {
+struct alignas(64) FaPagedParams {
+  CUtensorMap tm_k, tm_v;  // pages as [page][head][token][D], boxes of kPagedTile tokens (of a page, where it has fewer)
   KvView c;
   const void* q;
   void* o;
@@ -45,6 +48,7 @@ struct FaPagedParams {
   int row_limit;    // sequences with more query rows a KV head are not this kernel's
   FastDiv by_group;
   float scale_log2;
+  uint32_t* status;
   float* part_o;    // [2 * blocks][rows][D], O / l
   float* part_lse;  // [2 * blocks][rows], base 2
   PagedHead* heads; // [blocks]
@@ -60,13 +64,15 @@ struct FaPagedSmem {
   static constexpr int kTileBytes = kPagedTile * D;  // of keys, and of values
   static constexpr int kStages = D == 128 ? (kRows == 8 ? 2 : 3) : 3;
   static constexpr int kFrags = kRows / 8 * (D / 16);  // accumulator tiles of O^T
-  alignas(128) uint8_t ring[kPagedWarps][kStages][2 * kTileBytes];
+  alignas(1024) uint8_t ring[kPagedWarps][kStages][2 * kTileBytes];
   float4 o[kPagedWarps / 2][kFrags][32];   // a warp's accumulators, as its lanes hold them ...
   float ml[kPagedWarps / 2][2][kRows];     // ... and its maxima and sums
   alignas(16) float scales[kPagedWarps][kStages][4];  // keys, values of the tile's two halves; 0: a page that the cache does not have
+  uint64_t full[kPagedWarps][kStages];
   long long sums[kPagedWarps];
   long long found_at;
   int found;
+  uint32_t abort_flag;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -94,14 +100,9 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "r"(addr) : "memory");
   return w;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-// zeros where there is nothing to copy
-template <int kBytes>
-__device__ __forceinline__ void cp_async_if(uint32_t dst, const void* src, bool real) {
-  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+// four bytes, or zeros where there is nothing to copy
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -121,7 +122,7 @@ struct PagedCursor {
 __device__ __forceinline__ long long paged_list(const FaPagedParams& p, const KvSeq& s, int rows, int& tiles, int& row_tiles) {
   tiles = paged_tiles(s.len);
   row_tiles = static_cast<long long>(s.n) * p.group <= p.row_limit ? paged_row_tiles(s.n, p.group, rows) : 0;
-  return static_cast<long long>(tiles) * row_tiles * p.c.Hkv;
+  return static_cast<long long>(paged_places(tiles)) * row_tiles * p.c.Hkv;
 }
 __device__ __forceinline__ void paged_enter(const FaPagedParams& p, PagedCursor& at, int rows) {
   at.s = kv_seq(p.c, at.b);
@@ -150,6 +151,16 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const KvView& kv = p.c;
+  AbortCtx ctx{&sm.abort_flag, p.status};
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    for (int w = 0; w < kPagedWarps; ++w)
+      for (int i = 0; i < Smem::kStages; ++i) mbar_init(&sm.full[w][i], 1);
+    fence_mbar_init();
+    if ((smem_u32(smem_raw) & 1023u) != 0u) raise_abort(ctx, kStatusSmemMisaligned);
+    prefetch_tensormap(&p.tm_k);
+    prefetch_tensormap(&p.tm_v);
+  }
   grid_wait();
 
   // ---- this block's run of the list: the sequences' parts are added up in rounds of a block's threads
@@ -174,7 +185,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     }
   }
   const int run = blockIdx.x;
-  if (threadIdx.x == 0) p.heads[run].last = -1;
+  if (threadIdx.x == kPagedThreads - 32) p.heads[run].last = -1;  // the thread that may write another one
   if (run == 0) {
     for (int b = threadIdx.x; b < kv.B; b += kPagedThreads) {
       const uint32_t f = kv_seq_faults(kv, b);
@@ -220,89 +231,89 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   PagedCursor seg;  // the segment's item and first tile
   seg.b = sm.found;
   paged_enter(p, seg, kRows);
+  long long t = begin;  // place of the segment's first tile in the list
   {
-    const long long in = begin - sm.found_at, item = paged_div(in, seg.tiles);
-    seg.j = static_cast<int>(in - item * seg.tiles);
+    const int places = paged_places(seg.tiles);
+    const long long in = begin - sm.found_at, item = paged_div(in, places);
+    const int at = static_cast<int>(in - item * places);
+    seg.j = max(at - kPagedItemCost, 0);
+    t += max(kPagedItemCost - at, 0);
     seg.h = static_cast<int>(paged_div(item, seg.row_tiles));
     seg.rt = static_cast<int>(item - static_cast<long long>(seg.h) * seg.row_tiles);
   }
+  if (t >= end) return;  // a short run, all of it in front of an item's tiles
 
-  // ---- loads: the warp's next tile, and the ids of the pages of the one after
-  PagedCursor ld = seg;
-  long long ld_left = end - begin - warp;  // tiles of the run from the next load on; the warp's are every fourth
-  auto skip = [&](int tiles) {
-    ld.j += tiles;
-    while (ld.j >= ld.tiles && ld.b < kv.B) {
-      ld.j -= ld.tiles;
-      paged_next_item(p, ld, kRows);
+  // ---- the queries of a segment, as they come: columns 16 (c + 4 hh) .. + 15 of row g of each row tile
+  uint4 q_raw[kN][D / 64][2];
+  auto fetch_q = [&](const PagedCursor& at) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int row = at.rt * kRows + 8 * n + g;
+      const bool live = row < at.s.n * p.group;
+      const int tok = live ? fast_div(row, p.by_group) : 0, head = live ? row - tok * p.group : 0;
+      const T* src = static_cast<const T*>(p.q) + (at.s.start + tok) * p.q_st + (at.h * p.group + head) * p.q_sh + 16 * c;
+#pragma unroll
+      for (int hh = 0; hh < D / 64; ++hh) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q_raw[n][hh][e] = live ? *reinterpret_cast<const uint4*>(src + 64 * hh + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
+      }
     }
   };
-  auto pages = [&](int& first, int& second) {  // of the tile's halves; -1: none of the cache's, or behind the sequence
+  fetch_q(seg);  // in front of the tiles, which the memory takes its time over
+
+  // ---- loads: the warp's next tile, while the ids of the pages of the one after are on their way
+  PagedCursor ld = seg;
+  long long ld_left = end - t;  // places of the run from ld's tile on; the warp's tiles are every fourth
+  auto skip = [&](int tiles) {
+    ld.j += tiles;
+    ld_left -= tiles;
+    while (ld.j >= ld.tiles && ld_left > kPagedItemCost) {
+      ld.j -= ld.tiles;
+      ld_left -= kPagedItemCost;
+      paged_next_item(p, ld, kRows);
+    }
+    if (ld.j >= ld.tiles) ld_left = 0;
+  };
+  // of the tile's halves, as the table has them (-1: behind the sequence); looked at when they are used: a warp stops where it looks
+  // at what has not come yet
+  auto pages = [&](int& first, int& second) {
     const int tok = ld.j * kPagedTile;
-    first = tok < ld.s.len ? kv_page(kv, ld.b, tok >> kv.page_shift) : -1;
-    second = tok + 16 < ld.s.len ? kv_page(kv, ld.b, (tok + 16) >> kv.page_shift) : -1;
+    const int* row = kv.table + ld.b * kv.table_stride + (tok >> kv.page_shift);
+    first = second = -1;
+    if (tok < ld.s.len) first = row[0];
+    if (kv.page_shift == 4 && tok + 16 < ld.s.len) second = row[1];
   };
   int page0 = -1, page1 = -1;
-  if (ld_left > 0) {
-    skip(warp);
-    pages(page0, page1);
-  }
+  skip(warp);
+  if (ld_left > 0) pages(page0, page1);
   uint32_t ld_stage = 0;
-  // the lane's place in a copy: chunk of a row, row of a group
-  constexpr int kChunks = D / 16;
-  constexpr int kRowsAtOnce = 32 / kChunks;
-  constexpr int kCopies = 16 / kRowsAtOnce;  // of half a tile
-  const int ld_row = lane / kChunks;
-  uint32_t ld_dst[2];  // the swizzle of a row repeats every 8 rows (two copies at D = 128)
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = i * kRowsAtOnce + ld_row, chunk = lane % kChunks;
-    ld_dst[i] = row * D + (D == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) * 16;
-  }
-  const uint8_t* const ld_k = kv.k + kv_offset(ld_row, kv.k_ss) + lane % kChunks * 16;
-  const uint8_t* const ld_v = kv.v + kv_offset(ld_row, kv.v_ss) + lane % kChunks * 16;
-  const long long k_step = kv_offset(kRowsAtOnce, kv.k_ss), v_step = kv_offset(kRowsAtOnce, kv.v_ss);
-  auto load = [&]() {  // one tile, or nothing behind the run's end: a group of copies either way
+  const int no_page = max(kv.num_pages, 1);  // the first coordinate outside of the cache: the copy writes zeros
+  auto load = [&]() {                  // one tile, or nothing behind the run's end: a group of copies of scales either way
     if (ld_left > 0) {
-      const int tok = ld.j * kPagedTile;
-      const uint32_t base = smem_u32(sm.ring[warp][ld_stage]);
-      const int at = tok & ((1 << kv.page_shift) - 1);  // place of the tile's first key in its page
-      const bool full = tok + kPagedTile <= ld.s.len && page0 >= 0 && page1 >= 0;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int page = half == 0 ? page0 : page1;
-        const int place = half == 0 ? at : (kv.page_shift == 4 ? 0 : at + 16);
-        const uint8_t* ks = ld_k + kv_offset(page, kv.k_sp) + kv_offset(ld.h, kv.k_sh) + kv_offset(place, kv.k_ss);
-        const uint8_t* vs = ld_v + kv_offset(page, kv.v_sp) + kv_offset(ld.h, kv.v_sh) + kv_offset(place, kv.v_ss);
-        if (full) {
-#pragma unroll
-          for (int i = 0; i < kCopies; ++i, ks += k_step, vs += v_step) {
-            const uint32_t dst = base + half * 16 * D + ld_dst[i & 1] + (i >> 1) * 2 * kRowsAtOnce * D;
-            cp_async16(dst, ks);
-            cp_async16(dst + Smem::kTileBytes, vs);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kCopies; ++i, ks += k_step, vs += v_step) {
-            const uint32_t dst = base + half * 16 * D + ld_dst[i & 1] + (i >> 1) * 2 * kRowsAtOnce * D;
-            const bool real = page >= 0 && tok + half * 16 + i * kRowsAtOnce + ld_row < ld.s.len;
-            cp_async_if<16>(dst, real ? ks : kv.k, real);
-            cp_async_if<16>(dst + Smem::kTileBytes, real ? vs : kv.v, real);
-          }
-          if (lane == 0 && ((page0 < 0 && tok < ld.s.len) || (page1 < 0 && tok + 16 < ld.s.len))) kv_report(kv, HB_CACHE_BAD_PAGE);
+      const int tok = ld.j * kPagedTile, h = ld.h, len = ld.s.len, first = page0, second = page1;
+      skip(kPagedWarps);
+      if (ld_left > 0) pages(page0, page1);
+      const int a = static_cast<unsigned>(first) < static_cast<unsigned>(kv.num_pages) ? first : -1;
+      const int b = kv.page_shift > 4 ? a : static_cast<unsigned>(second) < static_cast<unsigned>(kv.num_pages) ? second : -1;
+      uint64_t* bar = &sm.full[warp][ld_stage];
+      uint8_t* dst = sm.ring[warp][ld_stage];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, 2 * Smem::kTileBytes);
+        const int at = tok & ((1 << kv.page_shift) - 1);  // place of the tile's first key in its page
+        tma_load_4d(dst, &p.tm_k, bar, 0, at, h, a < 0 ? no_page : a);
+        tma_load_4d(dst + Smem::kTileBytes, &p.tm_v, bar, 0, at, h, a < 0 ? no_page : a);
+        if (kv.page_shift == 4) {
+          tma_load_4d(dst + 16 * D, &p.tm_k, bar, 0, 0, h, b < 0 ? no_page : b);
+          tma_load_4d(dst + Smem::kTileBytes + 16 * D, &p.tm_v, bar, 0, 0, h, b < 0 ? no_page : b);
         }
+        if ((a < 0 && tok < len) || (b < 0 && tok + 16 < len)) kv_report(kv, HB_CACHE_BAD_PAGE);
       }
       if (lane < 4) {
-        const int page = lane & 1 ? page1 : page0;
-        const float* src = (lane & 2 ? kv.v_scale : kv.k_scale) + (page >= 0 ? static_cast<long long>(page) * kv.Hkv + ld.h : 0);
-        cp_async_if<4>(smem_u32(&sm.scales[warp][ld_stage][lane]), src, page >= 0);
+        const int page = lane & 1 ? b : a;
+        const float* src = (lane & 2 ? kv.v_scale : kv.k_scale) + (page >= 0 ? static_cast<long long>(page) * kv.Hkv + h : 0);
+        cp_async4(smem_u32(&sm.scales[warp][ld_stage][lane]), src, page >= 0);
       }
       if (++ld_stage == Smem::kStages) ld_stage = 0;
-      ld_left -= kPagedWarps;
-      if (ld_left > 0) {
-        skip(kPagedWarps);
-        pages(page0, page1);
-      }
     }
     cp_async_commit();
   };
@@ -324,10 +335,11 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   }
 
   // ---- segments
-  uint32_t stage = 0;
+  uint32_t stage = 0, phase = 0;
+  bool alive = true;  // until a wait gives up: then the block's barriers are all that is left to do
   int turn = 0;  // tiles of the run in front of the segment, modulo the warps
   bool first = true;
-  for (long long t = begin; t < end;) {
+  while (t < end) {
     const long long left = end - t;
     const int j0 = seg.j, j1 = left < seg.tiles - j0 ? j0 + static_cast<int>(left) : seg.tiles;
     const int rows = seg.s.n * p.group, row0 = seg.rt * kRows;
@@ -339,10 +351,6 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     int limit[kN][2];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int row = row0 + 8 * n + g;
-      const bool live = row < rows;
-      const int tok = live ? fast_div(row, p.by_group) : 0, head = live ? row - tok * p.group : 0;
-      const T* src = static_cast<const T*>(p.q) + (seg.s.start + tok) * p.q_st + (seg.h * p.group + head) * p.q_sh + 16 * c;
       float x[D / 64][16];
       float top = 0.f;
       bool finite = true;
@@ -350,8 +358,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       for (int hh = 0; hh < D / 64; ++hh) {
 #pragma unroll
         for (int e = 0; e < 16; e += 8) {
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (live) w = *reinterpret_cast<const uint4*>(src + 64 * hh + e);
+          const uint4 w = q_raw[n][hh][e >> 3];
           Pack2<T>::unpack(w.x, x[hh][e], x[hh][e + 1]);
           Pack2<T>::unpack(w.y, x[hh][e + 2], x[hh][e + 3]);
           Pack2<T>::unpack(w.z, x[hh][e + 4], x[hh][e + 5]);
@@ -397,7 +404,9 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
 
     for (int j = j0 + ((warp - turn) & (kPagedWarps - 1)); j < j1; j += kPagedWarps) {
       cp_async_wait<Smem::kStages - 2>();
-      __syncwarp();  // every lane's copies are there, and every lane is done with the tile before: its stage is free
+      alive = alive && mbar_wait_warp(&sm.full[warp][stage], phase, ctx, kRolePagedRows);
+      if (!alive) break;
+      __syncwarp();  // every lane's scales are there, and every lane is done with the tile before: its stage is free
       load();
       const uint32_t tile = smem_u32(sm.ring[warp][stage]);
       const float4 scales = *reinterpret_cast<const float4*>(sm.scales[warp][stage]);
@@ -514,6 +523,15 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
             vw[i][1] = w.y;
           }
         }
+        // what a page holds behind the sequence is loaded with it; as numbers it may be anything, and 0 times it has to be 0
+        if ((j + 1) * kPagedTile > seg.s.len) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = j * kPagedTile + 16 * t + 8 * (i >> 1) + ((2 * c + (i & 1)) ^ ((i & 1) << 2));
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) vw[i][w] = key < seg.s.len ? vw[i][w] : 0u;
+          }
+        }
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
 #pragma unroll
@@ -527,7 +545,18 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           }
         }
       }
-      if (++stage == Smem::kStages) stage = 0;
+      if (++stage == Smem::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    PagedCursor next = seg;
+    const long long last = t + (seg.tiles - 1 - j0);  // place of the item's last tile
+    const bool more = last + kPagedItemCost + 1 < end;
+    if (more) {
+      paged_next_item(p, next, kRows);
+      next.j = 0;
+      fetch_q(next);
     }
 
     // ---- the warps' results meet: 2 and 3 hand theirs to 0 and 1, 1 to 0, which stores the rows
@@ -629,22 +658,28 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         }
       }
     }
-    if (threadIdx.x == 0 && j0 == 0 && !whole) {
-      PagedHead& hd = p.heads[run];
-      hd.b = seg.b;
-      hd.h = seg.h;
-      hd.rt = seg.rt;
+    if (warp == kPagedWarps - 1 && lane == 0 && j0 == 0 && !whole) {
+      PagedHead hd;
+      hd.last = paged_run_of(total, runs, last);
       hd.slot = slot;
-      hd.last = paged_run_of(total, runs, t + seg.tiles - 1);
+      hd.h = seg.h;
+      hd.row0 = row0;
+      hd.start = seg.s.start;
+      hd.rows = rows;
+      p.heads[run] = hd;
     }
     __syncthreads();
     turn = (turn + (j1 - j0)) & (kPagedWarps - 1);
-    t += j1 - j0;
+    if (!more) break;
+    t = last + kPagedItemCost + 1;
     first = false;
-    seg.j = 0;
-    if (t < end) paged_next_item(p, seg, kRows);
+    seg = next;
   }
   cp_async_wait<0>();
+  if (!alive && lane == 0) {  // copies of this warp may be on their way into its ring: give them a while
+    for (int i = 0; i < Smem::kStages; ++i)
+      for (int spin = 0; spin < 4096 && !mbar_try_wait(&sm.full[warp][i], static_cast<uint32_t>(i) >= stage ? phase : phase ^ 1u); ++spin) {}
+  }
   grid_launch_dependents();
 }
 
@@ -660,9 +695,8 @@ __global__ void __launch_bounds__(32 * kPagedCombineWarps) fa_paged_combine_kern
   const int run = work / kRows, r = work - run * kRows;
   const PagedHead hd = p.heads[run];
   if (hd.last < 0) return;
-  const KvSeq s = kv_seq(p.c, hd.b);
-  const int row = hd.rt * kRows + r;
-  if (row >= s.n * p.group) return;
+  const int row = hd.row0 + r;
+  if (row >= hd.rows) return;
   auto slot_of = [&](int w) -> long long { return w == run ? hd.slot : 2 * w; };
 
   float top = -INFINITY;
@@ -709,11 +743,11 @@ __global__ void __launch_bounds__(32 * kPagedCombineWarps) fa_paged_combine_kern
 #pragma unroll
   for (int e = 0; e < kCols; e += 2) packed[e / 2] = Pack2<T>::pack(acc[e] * inv, acc[e + 1] * inv);
   const int tok = fast_div(row, p.by_group), head = hd.h * p.group + row - tok * p.group;
-  T* dst = static_cast<T*>(p.o) + (s.start + tok) * p.o_st + head * p.o_sh + lane * kCols;
+  T* dst = static_cast<T*>(p.o) + (hd.start + tok) * p.o_st + head * p.o_sh + lane * kCols;
   if constexpr (kCols == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
   else *reinterpret_cast<uint32_t*>(dst) = packed[0];
   if (lane == 0 && p.lse != nullptr)
-    p.lse[static_cast<long long>(s.start + tok) * p.Hq + head] = (sum != 0.f ? top + fast_log2(sum) : -INFINITY) * 0.6931471805599453f;
+    p.lse[static_cast<long long>(hd.start + tok) * p.Hq + head] = (sum != 0.f ? top + fast_log2(sum) : -INFINITY) * 0.6931471805599453f;
 }
 
 }  // namespace hb

@@ -31,9 +31,9 @@ const char* describe_status(uint32_t word) {
                          : role < 0x50 ? "attention backward" : "probe";
     static const char* const kFa[] = {"?", "softmax", "correction", "MMA issuer", "TMA producer", "drain",
                                       "split softmax", "split MMA issuer", "split TMA producer", "split drain",
-                                      "paged softmax", "paged MMA issuer", "paged producer", "paged drain"};
+                                      "paged softmax", "paged MMA issuer", "paged producer", "paged drain", "paged rows"};
     static const char* const kOther[] = {"?", "TMA producer", "MMA issuer", "consumer", "drain"};
-    const char* name = role < 14 ? kFa[role] : ((role & 0xfu) < 5 && role < 0x50) ? kOther[role & 0xfu] : "?";
+    const char* name = role < 15 ? kFa[role] : ((role & 0xfu) < 5 && role < 0x50) ? kOther[role & 0xfu] : "?";
     snprintf(buf, sizeof(buf),
              "status word 0x%x: a bounded wait of the %s kernel gave up (role 0x%x, %s); that launch's outputs are incomplete",
              word, kernel, role, name);
