@@ -75,20 +75,17 @@ static int launch_rows(const FaPagedParams& p, int blocks, cudaStream_t stream) 
     std::lock_guard<std::mutex> lock(g_paged_mutex);
     if (!configured[dev & 63]) {
       HB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)));
+      HB_CUDA_CHECK(cudaFuncSetAttribute(fa_paged_combine_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
       configured[dev & 63] = true;
     }
   }
   HB_CUDA_CHECK(launch_dependent(kernel, blocks, kPagedThreads, sizeof(Smem), stream, 0, p));
-  // parts of an item at most: a warp of the merge for every four
+  // parts of an item, where all items are alike
   const long long items = static_cast<long long>(p.c.B) * p.c.Hkv;
   const long long parts = (blocks + items - 1) / items + 1;
-  if (parts <= 8) {
-    const int per_block = kPagedCombineWarps;
-    HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, true>, blocks * kRows / per_block, 32 * per_block, 0, stream, 0, p, kRows));
-  } else {
-    const unsigned warps = static_cast<unsigned>(std::min<long long>(kPagedCombineWarps, (parts + 3) / 4));
-    HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D, false>, blocks * kRows, 32 * warps, 0, stream, 0, p, kRows));
-  }
+  const int warps = parts <= 6 ? 1 : parts <= 24 ? 2 : parts <= 64 ? 4 : kPagedCombineWarps;  // to a row
+  const int rows_here = warps == kPagedCombineWarps ? 1 : warps == 4 ? 4 : 8;
+  HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D>, blocks * (kRows / rows_here), 32 * warps * rows_here, 0, stream, 0, p, kRows, warps));
   return HB_OK;
 }
 template <typename T>

@@ -683,61 +683,76 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   grid_launch_dependents();
 }
 
-// Merges the parts of an item, a row a warp-group: its warps deal the parts out, a lane has D / 32 columns; weights 2^(lse - max).  Where
-// items are in many parts a block has one row, and a warp for every four parts; elsewhere a warp goes over its row's parts alone,
-// and a block has a row for every warp: a decode step of many sequences has a few hundred items in parts, not thousands of blocks.
-constexpr int kPagedCombineWarps = 8;
-template <typename T, int D, bool kAlone>
-__global__ void __launch_bounds__(32 * kPagedCombineWarps) fa_paged_combine_kernel(const __grid_constant__ FaPagedParams p, int kRows) {
+// Merges the parts of the items that are in any: a block has some rows of one run's head, `warps` warps deal a row's parts out
+// between them, a lane has D / 32 columns; weights 2^(lse - max).  What it costs is its chain of loads (head, parts) and the blocks
+// that find nothing to do: a block for every row was 3552 of them for 24 items in 18 parts each (B3 Hq64 Hkv8 60011 keys).
+constexpr int kPagedCombineWarps = 16;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kPagedCombineWarps) fa_paged_combine_kernel(const __grid_constant__ FaPagedParams p, int kRows, int warps) {
+  grid_launch_dependents();
   grid_wait();
-  const int warp = kAlone ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kAlone ? 1 : blockDim.x >> 5;
-  const int work = kAlone ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x);
-  const int run = work / kRows, r = work - run * kRows;
+  constexpr int kCols = D / 32, kAhead = 4;
+  const int rows_here = (blockDim.x >> 5) / warps, blocks_of_run = kRows / rows_here;
+  const int run = blockIdx.x / blocks_of_run;
   const PagedHead hd = p.heads[run];
   if (hd.last < 0) return;
-  const int row = hd.row0 + r;
-  if (row >= hd.rows) return;
-  auto slot_of = [&](int w) -> long long { return w == run ? hd.slot : 2 * w; };
-
+  const int warp = uniform_warp(), lane = threadIdx.x & 31, part0 = warp % warps;
+  const int r = (blockIdx.x - run * blocks_of_run) * rows_here + warp / warps, row = hd.row0 + r;
+  const bool live = row < hd.rows;
+  const int parts = live ? hd.last - run + 1 : 0;
+  auto at = [&](int part) -> long long { return static_cast<long long>(part == 0 ? hd.slot : 2 * (run + part)) * kRows + r; };
+  auto values = [&](int part, float (&x)[kCols]) {
+    const float* src = p.part_o + at(part) * D + lane * kCols;
+    if constexpr (kCols == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(src);
+      x[0] = y.x;
+      x[1] = y.y;
+      x[2] = y.z;
+      x[3] = y.w;
+    } else {
+      const float2 y = *reinterpret_cast<const float2*>(src);
+      x[0] = y.x;
+      x[1] = y.y;
+    }
+  };
+  float ahead[kAhead][kCols];  // the first parts' values are on their way with the weights
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (part0 + i * warps < parts) values(part0 + i * warps, ahead[i]);
   float top = -INFINITY;
-  for (int w = run + lane; w <= hd.last; w += 32) top = fmaxf(top, p.part_lse[slot_of(w) * kRows + r]);
+  for (int part = lane; part < parts; part += 32) top = fmaxf(top, p.part_lse[at(part)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (top == -INFINITY) top = 0.f;
-
-  constexpr int kCols = D / 32;
   float acc[kCols] = {}, sum = 0.f;
-#pragma unroll 4
-  for (int w = run + warp; w <= hd.last; w += warps) {
-    const long long at = slot_of(w) * kRows + r;
-    const float wt = fast_exp2(p.part_lse[at] - top);
-    const float* src = p.part_o + at * D + lane * kCols;
-    sum += wt;
-    if constexpr (kCols == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(src);
-      acc[0] += wt * x.x;
-      acc[1] += wt * x.y;
-      acc[2] += wt * x.z;
-      acc[3] += wt * x.w;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(src);
-      acc[0] += wt * x.x;
-      acc[1] += wt * x.y;
+  for (int part = part0; part < parts; part += kAhead * warps) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int mine = part + i * warps;
+      if (mine >= parts) continue;
+      const float wt = fast_exp2(p.part_lse[at(mine)] - top);
+      sum += wt;
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) acc[e] = fmaf(wt, ahead[i][e], acc[e]);
     }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (part + (kAhead + i) * warps < parts) values(part + (kAhead + i) * warps, ahead[i]);
   }
-  if constexpr (!kAlone) {
+  if (warps > 1) {
     __shared__ float s_acc[kPagedCombineWarps][D], s_sum[kPagedCombineWarps];
 #pragma unroll
     for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    if (warp != 0) return;
+    if (part0 != 0) return;
     for (int k = 1; k < warps; ++k) {
-      sum += s_sum[k];
+      sum += s_sum[warp + k];
 #pragma unroll
-      for (int e = 0; e < kCols; ++e) acc[e] += s_acc[k][lane * kCols + e];
+      for (int e = 0; e < kCols; ++e) acc[e] += s_acc[warp + k][lane * kCols + e];
     }
   }
+  if (!live) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   uint32_t packed[kCols / 2];
 #pragma unroll
