@@ -52,14 +52,23 @@ static int paged_blocks(const hb_fa_paged_args* a, int sm_count) {
   return runs < most ? (int)runs : most;
 }
 
-// Which kernels a call takes.  The tiles kernel has the sequences of more than kPagedRowLimit query rows a KV head, the rows kernel the
+// Which kernels a call takes.  The tiles kernel has the sequences of more than paged_row_limit query rows a KV head, the rows kernel the
 // others; where the call says that there are none of the former (or all are), the other one is not launched.
-constexpr int kPagedRowLimit = 64;
-static bool paged_takes_tiles(const hb_fa_paged_args* a) { return paged_most_rows(a) > kPagedRowLimit; }
-static bool paged_takes_rows(const hb_fa_paged_args* a) { return a->cache.starts != nullptr || !paged_takes_tiles(a); }
+static int paged_row_limit(const hb_fa_paged_args* a, int sm_count) {
+  const double items = (double)a->cache.B * a->cache.Hkv;
+  int limit = kPagedMaxRows;
+  for (int tiles = 2; tiles <= 64; ++tiles) {
+    const double rows_cost = items * tiles / sm_count * 375;
+    const double tiles_cost = std::ceil(items * ((tiles * kPagedMaxRows + kPagedBlockRows - 1) / kPagedBlockRows) / sm_count) * 850;
+    if (rows_cost <= tiles_cost) limit = tiles * kPagedMaxRows;
+  }
+  return limit;
+}
+static bool paged_takes_tiles(const hb_fa_paged_args* a, int sm_count) { return paged_most_rows(a) > paged_row_limit(a, sm_count); }
+static bool paged_takes_rows(const hb_fa_paged_args* a, int sm_count) { return a->cache.starts != nullptr || !paged_takes_tiles(a, sm_count); }
 
 static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
-  if (!paged_takes_rows(a)) return 0;
+  if (!paged_takes_rows(a, sm_count)) return 0;
   const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
   return 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
 }
@@ -80,18 +89,26 @@ static int launch_rows(const FaPagedParams& p, int blocks, cudaStream_t stream) 
     }
   }
   HB_CUDA_CHECK(launch_dependent(kernel, blocks, kPagedThreads, sizeof(Smem), stream, 0, p));
+  return HB_OK;
+}
+template <typename T, int D>
+static int launch_combine(const FaPagedParams& p, int rows, int blocks, cudaStream_t stream) {
   // parts of an item, where all items are alike
   const long long items = static_cast<long long>(p.c.B) * p.c.Hkv;
   const long long parts = (blocks + items - 1) / items + 1;
   const int warps = parts <= 6 ? 1 : parts <= 24 ? 2 : parts <= 64 ? 4 : kPagedCombineWarps;  // to a row
   const int rows_here = warps == kPagedCombineWarps ? 1 : warps == 4 ? 4 : 8;
-  HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D>, blocks * (kRows / rows_here), 32 * warps * rows_here, 0, stream, 0, p, kRows, warps));
+  HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D>, blocks * (rows / rows_here), 32 * warps * rows_here, 0, stream, 0, p, rows, warps));
   return HB_OK;
 }
 template <typename T>
 static int launch_rows_of(const FaPagedParams& p, int D, int rows, int blocks, cudaStream_t stream) {
   if (D == 128) return rows == 8 ? launch_rows<T, 128, 8>(p, blocks, stream) : launch_rows<T, 128, 16>(p, blocks, stream);
   return rows == 8 ? launch_rows<T, 64, 8>(p, blocks, stream) : launch_rows<T, 64, 16>(p, blocks, stream);
+}
+template <typename T>
+static int launch_combine_of(const FaPagedParams& p, int D, int rows, int blocks, cudaStream_t stream) {
+  return D == 128 ? launch_combine<T, 128>(p, rows, blocks, stream) : launch_combine<T, 64>(p, rows, blocks, stream);
 }
 
 template <typename T, int D>
@@ -119,11 +136,11 @@ static int launch_tiles_of(const FaPagedTilesParams& p, int D, unsigned grid, in
 }
 
 // Blocks of the tiles kernel: exactly the items, or where the device knows only, as many as so many rows can be.
-static int64_t paged_tiles_grid(const hb_fa_paged_args* a) {
+static int64_t paged_tiles_grid(const hb_fa_paged_args* a, int sm_count) {
   const hb_kv_cache& c = a->cache;
   const int64_t group = a->Hq / c.Hkv, rows = group * c.T;
   if (c.starts == nullptr) return static_cast<int64_t>(c.B) * c.Hkv * ((rows / c.B + kPagedBlockRows - 1) / kPagedBlockRows);
-  return c.Hkv * (rows / kPagedBlockRows + std::min<int64_t>(c.B, rows / (kPagedRowLimit + 1)));
+  return c.Hkv * (rows / kPagedBlockRows + std::min<int64_t>(c.B, rows / (paged_row_limit(a, sm_count) + 1)));
 }
 
 }  // namespace hb
@@ -152,6 +169,7 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != HB_OK) return rc;
+  if (paged_tiles_grid(a, st->sm_count) > 0x7fffffffll) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
   const uint64_t need = paged_workspace(a, st->sm_count);
   if (need > 0 && (workspace == nullptr || bytes < need))
     return set_error(HB_ERR_BAD_ARG, "hb_fa_paged: needs a workspace of %llu bytes, got %llu", (unsigned long long)need,
@@ -175,39 +193,45 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
     p.by_group = make_fast_div(p.group);
     p.scale_log2 = scale * 1.4426950408889634f;
   };
-  if (paged_takes_tiles(a)) {
-    const int64_t grid = paged_tiles_grid(a);
-    if (grid > 0x7fffffffll) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
-    FaPagedTilesParams p;
+  const int sm_count = st->sm_count;
+  const bool take_rows = paged_takes_rows(a, sm_count), take_tiles = paged_takes_tiles(a, sm_count);
+  FaPagedParams p;
+  const int rows = paged_tile_rows(a), blocks = paged_blocks(a, sm_count);
+  if (take_rows) {
     fill(p);
-    p.row_limit = kPagedRowLimit;
+    p.row_limit = take_tiles ? paged_row_limit(a, sm_count) : INT_MAX;
+    p.chained = take_tiles ? 1 : 0;
     p.status = st->status_word;
+    for (const bool keys : {true, false}) {
+      // an axis of one page, head or token may carry any stride
+      const uint64_t dims[4] = {(uint64_t)c.D, (uint64_t)c.page_size, (uint64_t)c.Hkv, (uint64_t)std::max(c.num_pages, 1)};
+      const int64_t given[3] = {keys ? c.k_stride_s : c.v_stride_s, keys ? c.k_stride_h : c.v_stride_h, keys ? c.k_stride_p : c.v_stride_p};
+      uint64_t strides[3];
+      for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (uint64_t)given[i] : (uint64_t)c.D;
+      const uint32_t box[4] = {(uint32_t)c.D, (uint32_t)std::min(c.page_size, kPagedTile), 1, 1};
+      rc = encode_tensor_map(keys ? &p.tm_k : &p.tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box,
+                             c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+      if (rc != HB_OK) return rc;
+    }
+    p.heads = static_cast<PagedHead*>(workspace);
+    p.part_o = reinterpret_cast<float*>(p.heads + blocks);
+    p.part_lse = p.part_o + 2ll * blocks * rows * c.D;
+    rc = a->dtype == HB_BF16 ? launch_rows_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_rows_of<__half>(p, c.D, rows, blocks, stream);
+    if (rc != HB_OK) return rc;
+  }
+  if (take_tiles) {
+    const int64_t grid = paged_tiles_grid(a, sm_count);
+    FaPagedTilesParams t;
+    fill(t);
+    t.row_limit = paged_row_limit(a, sm_count);
+    t.chained = take_rows ? 1 : 0;
+    t.status = st->status_word;
     if (grid > 0) {
-      rc = a->dtype == HB_BF16 ? launch_tiles_of<__nv_bfloat16>(p, c.D, static_cast<unsigned>(grid), st->smem_optin, stream)
-                               : launch_tiles_of<__half>(p, c.D, static_cast<unsigned>(grid), st->smem_optin, stream);
+      rc = a->dtype == HB_BF16 ? launch_tiles_of<__nv_bfloat16>(t, c.D, static_cast<unsigned>(grid), st->smem_optin, stream)
+                               : launch_tiles_of<__half>(t, c.D, static_cast<unsigned>(grid), st->smem_optin, stream);
       if (rc != HB_OK) return rc;
     }
   }
-  if (!paged_takes_rows(a)) return HB_OK;
-  const int rows = paged_tile_rows(a), blocks = paged_blocks(a, st->sm_count);
-  FaPagedParams p;
-  fill(p);
-  p.row_limit = paged_takes_tiles(a) ? kPagedRowLimit : INT_MAX;
-  p.status = st->status_word;
-  for (const bool keys : {true, false}) {
-    // an axis of one page, head or token may carry any stride
-    const uint64_t dims[4] = {(uint64_t)c.D, (uint64_t)c.page_size, (uint64_t)c.Hkv, (uint64_t)std::max(c.num_pages, 1)};
-    const int64_t given[3] = {keys ? c.k_stride_s : c.v_stride_s, keys ? c.k_stride_h : c.v_stride_h, keys ? c.k_stride_p : c.v_stride_p};
-    uint64_t strides[3];
-    for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (uint64_t)given[i] : (uint64_t)c.D;
-    const uint32_t box[4] = {(uint32_t)c.D, (uint32_t)std::min(c.page_size, kPagedTile), 1, 1};
-    rc = encode_tensor_map(keys ? &p.tm_k : &p.tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box,
-                           c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-    if (rc != HB_OK) return rc;
-  }
-  p.heads = static_cast<PagedHead*>(workspace);
-  p.part_o = reinterpret_cast<float*>(p.heads + blocks);
-  p.part_lse = p.part_o + 2ll * blocks * rows * c.D;
-  return a->dtype == HB_BF16 ? launch_rows_of<__nv_bfloat16>(p, c.D, rows, blocks, stream)
-                             : launch_rows_of<__half>(p, c.D, rows, blocks, stream);
+  if (!take_rows) return HB_OK;
+  return a->dtype == HB_BF16 ? launch_combine_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_combine_of<__half>(p, c.D, rows, blocks, stream);
 }

@@ -29,6 +29,7 @@ struct FaPagedTilesParams {
   long long q_st, q_sh, o_st, o_sh;
   int Hq, group, causal;
   int row_limit;  // sequences with no more query rows a KV head are the rows kernel's
+  int chained;    // the rows kernel of the same call runs in front, and beside this one
   FastDiv by_group;
   float scale_log2;
   uint32_t* status;
@@ -467,14 +468,21 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
     if ((smem_u32(smem_raw) & 1023u) != 0u) raise_abort(ctx, kStatusSmemMisaligned);
   }
   __syncthreads();
-  grid_wait();
+  // The rows kernel lets this one in behind its own wait: all that is earlier is complete then, and the two write rows of different
+  // sequences.  Whoever waits for this kernel has both: it waits for the rows kernel at its end.
+  if (!p.chained) grid_wait();
 
-  // ---- the block's item: sequences in order, within one the last 256 rows (which see most keys) of every KV head first
+  // ---- the block's item: the last 256 rows (which see most keys) of every KV head first, where sequences are alike of all of
+  // them; sequences in order elsewhere
   PagedItem it;
   {
     const KvView& kv = p.c;
     long long before = 0;
-    for (int b0 = 0; b0 < kv.B && before <= blockIdx.x; b0 += kPagedTilesThreads) {
+    if (kv.starts == nullptr && threadIdx.x == 0) {
+      s.found = 0;
+      s.found_at = 0;
+    }
+    for (int b0 = kv.starts == nullptr ? kv.B : 0; b0 < kv.B && before <= blockIdx.x; b0 += kPagedTilesThreads) {
       const int b = b0 + threadIdx.x;
       const long long own = b < kv.B ? static_cast<long long>(paged_blocks_of(p, kv_seq(kv, b))) * kv.Hkv : 0;
       long long upto = own;
@@ -503,11 +511,20 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
       }
     }
     __syncthreads();
-    if (s.found < 0) return;  // the grid is cut for the most items that so many rows can be
+    if (s.found < 0) {  // the grid is cut for the most items that so many rows can be
+      if (p.chained) grid_wait();
+      return;
+    }
     it.b = s.found;
-    it.s = kv_seq(kv, it.b);
-    const int in = static_cast<int>(blockIdx.x - s.found_at), rank = in / kv.Hkv;
+    const int in = static_cast<int>(blockIdx.x - s.found_at);
+    int rank = in / kv.Hkv;
     it.h = in - rank * kv.Hkv;
+    if (kv.starts == nullptr) {
+      const int turn = rank / kv.B;
+      it.b = rank - turn * kv.B;
+      rank = turn;
+    }
+    it.s = kv_seq(kv, it.b);
     it.rows = it.s.n * p.group;
     it.row0 = (paged_blocks_of(p, it.s) - 1 - rank) * kPagedBlockRows;
     const int tiles = max((it.s.len + kTileN - 1) / kTileN, 1);
@@ -555,6 +572,7 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
   }
   __syncwarp();
   tc_fence_before();
+  if (p.chained) grid_wait();
   grid_launch_dependents();
   __syncthreads();
   if (warp == 8) {
