@@ -54,23 +54,60 @@ static int paged_blocks(const hb_fa_paged_args* a, int sm_count) {
 
 // Which kernels a call takes.  The tiles kernel has the sequences of more than paged_row_limit query rows a KV head, the rows kernel the
 // others; where the call says that there are none of the former (or all are), the other one is not launched.
+// The limit is where 32 keys cost the SMs as much either way, all sequences taken alike: in the rows kernel 375 cycles for every 16 rows,
+// dealt out evenly; in the tiles kernel 850 for up to 256, by rounds of whole blocks, or, where items are dealt out to several
+// blocks, divided by 0.6 of their number, which is what their starts and the merge leave of it.  us, rows kernel | tiles kernel, 4096 keys, Hq32 Hkv8: B1 64 rows (a KV head) 22
+// | 30, 256 rows 42 | 29; B4 48 rows 33 | 38, 128 rows 62 | 39; B16 32 rows 60 | 72, 48 rows 83 | 73; B64 32 rows 199 | 273, 48 rows 291 | 274.
+static int paged_splits_of(double items, double tiles, int sm_count);
+static double paged_most_tiles(const hb_fa_paged_args* a);
 static int paged_row_limit(const hb_fa_paged_args* a, int sm_count) {
   const double items = (double)a->cache.B * a->cache.Hkv;
   int limit = kPagedMaxRows;
-  for (int tiles = 2; tiles <= 64; ++tiles) {
+  for (int tiles = 2; tiles <= 256; ++tiles) {
+    const double blocks = items * ((tiles * kPagedMaxRows + kPagedBlockRows - 1) / kPagedBlockRows);
+    const int splits = paged_splits_of(blocks, paged_most_tiles(a), sm_count);
     const double rows_cost = items * tiles / sm_count * 375;
-    const double tiles_cost = std::ceil(items * ((tiles * kPagedMaxRows + kPagedBlockRows - 1) / kPagedBlockRows) / sm_count) * 850;
-    if (rows_cost <= tiles_cost) limit = tiles * kPagedMaxRows;
+    const double tiles_cost = 850 * (splits > 1 ? 1 / std::max(1.0, 0.6 * splits) : std::ceil(blocks / sm_count));
+    if (rows_cost > tiles_cost) break;
+    limit = tiles * kPagedMaxRows;
   }
   return limit;
 }
 static bool paged_takes_tiles(const hb_fa_paged_args* a, int sm_count) { return paged_most_rows(a) > paged_row_limit(a, sm_count); }
 static bool paged_takes_rows(const hb_fa_paged_args* a, int sm_count) { return a->cache.starts != nullptr || !paged_takes_tiles(a, sm_count); }
 
+// Items of the tiles kernel: exactly, or where the device knows only, as many as so many rows can be.
+static int64_t paged_items(const hb_fa_paged_args* a, int sm_count) {
+  const hb_kv_cache& c = a->cache;
+  const int64_t group = a->Hq / c.Hkv, rows = group * c.T;
+  if (c.starts == nullptr) return static_cast<int64_t>(c.B) * c.Hkv * ((rows / c.B + kPagedBlockRows - 1) / kPagedBlockRows);
+  return c.Hkv * (rows / kPagedBlockRows + std::min<int64_t>(c.B, rows / (paged_row_limit(a, sm_count) + 1)));
+}
+// Blocks for an item: as many as one round of blocks has place for, up to 16, each with three tiles at least of those that the page
+// table has room for.  More rounds of smaller blocks cost more than they even out, since a block's start and end take about as long as
+// five tiles.  us with 1 | 2 | 4 | 8 blocks an item: B1 Hq32 Hkv8, 128 rows, 4096 keys (16 items) 78.5 | 49.6 | 34.6 | 32.2; 512 rows (64 items) 79 | 55
+// | 65 | 91; B1 Hq32 Hkv2, 128 rows, 20000 keys (16 items) 340 | 182 | 101 | 67; B4, 256 rows (128 items) 80 | 102 | 129 | 178.
+constexpr int kPagedMaxSplits = 16;
+static int paged_splits_of(double items, double tiles, int sm_count) {
+  return static_cast<int>(std::max(1.0, std::min({sm_count / std::max(items, 1.0), tiles / 3, (double)kPagedMaxSplits})));
+}
+static double paged_most_tiles(const hb_fa_paged_args* a) { return (double)a->cache.max_pages * a->cache.page_size / kTileN; }
+static int paged_splits(const hb_fa_paged_args* a, int sm_count) {
+  return paged_splits_of((double)paged_items(a, sm_count), paged_most_tiles(a), sm_count);
+}
+static uint64_t paged_tiles_workspace(const hb_fa_paged_args* a, int sm_count) {
+  if (!paged_takes_tiles(a, sm_count)) return 0;
+  const uint64_t splits = paged_splits(a, sm_count), items = paged_items(a, sm_count);
+  return splits > 1 ? items * (sizeof(PagedParts) + splits * kPagedBlockRows * (a->cache.D + 1) * sizeof(float)) : 0;
+}
+
 static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
-  if (!paged_takes_rows(a, sm_count)) return 0;
-  const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
-  return 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
+  uint64_t bytes = paged_tiles_workspace(a, sm_count);
+  if (paged_takes_rows(a, sm_count)) {
+    const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
+    bytes += 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
+  }
+  return bytes;
 }
 
 template <typename T, int D, int kRows>
@@ -135,14 +172,6 @@ static int launch_tiles_of(const FaPagedTilesParams& p, int D, unsigned grid, in
   return D == 128 ? launch_tiles<T, 128>(p, grid, smem_optin, stream) : launch_tiles<T, 64>(p, grid, smem_optin, stream);
 }
 
-// Blocks of the tiles kernel: exactly the items, or where the device knows only, as many as so many rows can be.
-static int64_t paged_tiles_grid(const hb_fa_paged_args* a, int sm_count) {
-  const hb_kv_cache& c = a->cache;
-  const int64_t group = a->Hq / c.Hkv, rows = group * c.T;
-  if (c.starts == nullptr) return static_cast<int64_t>(c.B) * c.Hkv * ((rows / c.B + kPagedBlockRows - 1) / kPagedBlockRows);
-  return c.Hkv * (rows / kPagedBlockRows + std::min<int64_t>(c.B, rows / (paged_row_limit(a, sm_count) + 1)));
-}
-
 }  // namespace hb
 
 extern "C" int hb_fa_paged_workspace(const hb_fa_paged_args* a, uint64_t* bytes) {
@@ -169,7 +198,7 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != HB_OK) return rc;
-  if (paged_tiles_grid(a, st->sm_count) > 0x7fffffffll) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
+  if (paged_items(a, st->sm_count) > 0x7fffffffll / (kPagedBlockRows / 32)) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
   const uint64_t need = paged_workspace(a, st->sm_count);
   if (need > 0 && (workspace == nullptr || bytes < need))
     return set_error(HB_ERR_BAD_ARG, "hb_fa_paged: needs a workspace of %llu bytes, got %llu", (unsigned long long)need,
@@ -213,25 +242,41 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
                              c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
       if (rc != HB_OK) return rc;
     }
-    p.heads = static_cast<PagedHead*>(workspace);
+    p.heads = reinterpret_cast<PagedHead*>(static_cast<uint8_t*>(workspace) + paged_tiles_workspace(a, sm_count));
     p.part_o = reinterpret_cast<float*>(p.heads + blocks);
     p.part_lse = p.part_o + 2ll * blocks * rows * c.D;
     rc = a->dtype == HB_BF16 ? launch_rows_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_rows_of<__half>(p, c.D, rows, blocks, stream);
     if (rc != HB_OK) return rc;
   }
-  if (take_tiles) {
-    const int64_t grid = paged_tiles_grid(a, sm_count);
-    FaPagedTilesParams t;
+  FaPagedTilesParams t;
+  const int64_t items = paged_items(a, sm_count);
+  if (take_tiles && items > 0) {
     fill(t);
     t.row_limit = paged_row_limit(a, sm_count);
     t.chained = take_rows ? 1 : 0;
     t.status = st->status_word;
-    if (grid > 0) {
-      rc = a->dtype == HB_BF16 ? launch_tiles_of<__nv_bfloat16>(t, c.D, static_cast<unsigned>(grid), st->smem_optin, stream)
-                               : launch_tiles_of<__half>(t, c.D, static_cast<unsigned>(grid), st->smem_optin, stream);
-      if (rc != HB_OK) return rc;
-    }
+    t.splits = paged_splits(a, sm_count);
+    t.parts = static_cast<PagedParts*>(workspace);
+    t.part_o = t.splits > 1 ? reinterpret_cast<float*>(t.parts + items) : nullptr;
+    t.part_lse = t.splits > 1 ? t.part_o + items * t.splits * kPagedBlockRows * c.D : nullptr;
+    const unsigned grid = static_cast<unsigned>(items * t.splits);
+    rc = a->dtype == HB_BF16 ? launch_tiles_of<__nv_bfloat16>(t, c.D, grid, st->smem_optin, stream)
+                             : launch_tiles_of<__half>(t, c.D, grid, st->smem_optin, stream);
+    if (rc != HB_OK) return rc;
   }
-  if (!take_rows) return HB_OK;
-  return a->dtype == HB_BF16 ? launch_combine_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_combine_of<__half>(p, c.D, rows, blocks, stream);
+  if (take_rows) {
+    rc = a->dtype == HB_BF16 ? launch_combine_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_combine_of<__half>(p, c.D, rows, blocks, stream);
+    if (rc != HB_OK) return rc;
+  }
+  if (!take_tiles || items == 0 || t.splits == 1) return HB_OK;
+  const unsigned grid = static_cast<unsigned>(items * (kPagedBlockRows / 32));
+  cudaError_t err;
+  if (a->dtype == HB_BF16)
+    err = c.D == 128 ? launch_dependent(fa_paged_tiles_combine_kernel<__nv_bfloat16, 128>, grid, 256, 0, stream, 0, t)
+                     : launch_dependent(fa_paged_tiles_combine_kernel<__nv_bfloat16, 64>, grid, 256, 0, stream, 0, t);
+  else
+    err = c.D == 128 ? launch_dependent(fa_paged_tiles_combine_kernel<__half, 128>, grid, 256, 0, stream, 0, t)
+                     : launch_dependent(fa_paged_tiles_combine_kernel<__half, 64>, grid, 256, 0, stream, 0, t);
+  HB_CUDA_CHECK(err);
+  return HB_OK;
 }

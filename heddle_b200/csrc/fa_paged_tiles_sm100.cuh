@@ -8,6 +8,8 @@
 //   - the scales of a tile's pages are taken relative to the tile's largest, powers of two that fp16 holds beside the code; where all
 //     are alike, nearly always, nothing is multiplied.  The largest goes into the factor of the scores and the unit of P';
 //   - queries are scaled into fp16 by a power of two for each row, by the thread that owns the row.
+// An item's key tiles are dealt out to several blocks where items are few, or do not fill the SMs evenly (paged_splits); their fp32 partial
+// results meet in fa_paged_tiles_combine_kernel.
 // A row's maximum is adopted when it grew by more than 2^7, and O's unit when a tile has a larger value scale: P' = 256 P
 // (scale / unit).  O is rescaled by the row's own thread, as in fa_split.
 #pragma once
@@ -33,6 +35,15 @@ struct FaPagedTilesParams {
   FastDiv by_group;
   float scale_log2;
   uint32_t* status;
+  int splits;       // blocks of the grid for an item: each has a part of its key tiles
+  float* part_o;    // splits > 1: [grid][256][D], O / l of the part
+  float* part_lse;  // [grid][256], base 2; -inf: no keys
+  struct PagedParts* parts;  // [grid / splits]
+};
+
+struct alignas(16) PagedParts {  // of an item
+  int count;                // 0: no item, 1: its block has stored the rows
+  int h, row0, rows, start, pad[3];
 };
 
 template <int D>
@@ -60,7 +71,9 @@ struct FaPagedTilesSmem {
 struct PagedItem {
   KvSeq s;
   int b, h, row0, rows;  // rows of the sequence in this KV head
-  int n[2];              // key tiles of the two row tiles, 0: no rows
+  int j0, j1;            // key tiles of the block
+  int n[2];              // of them, row tile i has [j0, n[i])
+  bool whole;            // all of the item's
 };
 
 __device__ __forceinline__ int paged_blocks_of(const FaPagedTilesParams& p, const KvSeq& s) {
@@ -76,7 +89,11 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const uint32_t tS = tmem + lane_off + static_cast<uint32_t>(i * kTileN), tO = tmem + lane_off + 256u + static_cast<uint32_t>(i * 128);
   const int n = i == 0 ? it.n[0] : it.n[1];
-  if (n == 0) return;
+  const long long part_row = static_cast<long long>(blockIdx.x) * kPagedBlockRows + kTileM * i + r;
+  if (n <= it.j0) {
+    if (!it.whole) p.part_lse[part_row] = -INFINITY;
+    return;
+  }
   const int first = it.row0 + kTileM * i, row = first + r;
   const bool live = row < it.rows;
   const int tok = live ? fast_div(row, p.by_group) : 0, head = it.h * p.group + (live ? row - tok * p.group : 0);
@@ -123,14 +140,15 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   }
 
   float m = -INFINITY, l = 0.f, v_unit = 0.f;
-  for (int j = 0; j < n; ++j) {
-    if (!mbar_wait_warp(&s.s_full[i], j & 1, ctx, kRolePagedSoftmax)) return;
+  for (int j = it.j0; j < n; ++j) {
+    const int at = j - it.j0;
+    if (!mbar_wait_warp(&s.s_full[i], at & 1, ctx, kRolePagedSoftmax)) return;
     tc_fence_after();
     uint32_t v[kTileN];
 #pragma unroll
     for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, &v[c * 32]);
-    if (!mbar_wait_warp(&s.meta_full[j % Smem::kMeta], (j / Smem::kMeta) & 1, ctx, kRolePagedSoftmax)) return;
-    const float4 meta = s.meta[j % Smem::kMeta];
+    if (!mbar_wait_warp(&s.meta_full[at % Smem::kMeta], (at / Smem::kMeta) & 1, ctx, kRolePagedSoftmax)) return;
+    const float4 meta = s.meta[at % Smem::kMeta];
     const uint32_t gone = __float_as_uint(meta.z);
     tmem_wait_ld();
 
@@ -197,7 +215,7 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     unpack_f32x2(sb, sum2, sum3);
     l = fmaf((sum0 + sum1) + (sum2 + sum3), __int_as_float((127 - e) << 23), l);
     // S(j) was committed behind P V(j - 1), so that product is complete, and P V(j) is only issued after this warp's arrival
-    if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+    if (at > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -217,23 +235,28 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   if (!mbar_wait_warp(&s.o_full[i], 0, ctx, kRolePagedSoftmax)) return;
   tc_fence_after();
   const float inv = l != 0.f ? v_unit * (1.f / 256.f) / l : 0.f;  // a row without keys is 0, one with a NaN is NaN
+  const float lse2 = l != 0.f ? (m == -INFINITY ? 0.f : m) + fast_log2(l) : -INFINITY;
   T* dst = static_cast<T*>(p.o) + static_cast<long long>(it.s.start + tok) * p.o_st + head * p.o_sh;
+  float* part = p.part_o + (part_row - (r & 3)) * D;
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
     uint32_t o[32];
     __syncwarp();
     tmem_ld32(tO + c * 32, o);
     tmem_wait_ld();
-    uint4 w[4];
-    pack_row32<T>(o, inv, w);
-    if (live) {
+    if (it.whole) {
+      uint4 w[4];
+      pack_row32<T>(o, inv, w);
+      if (live) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(dst + c * 32 + k * 8) = w[k];
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(dst + c * 32 + k * 8) = w[k];
+      }
+    } else {
+      store_rows32_f32(part + c * 32, D, 4, o, inv);
     }
   }
-  if (live && p.lse != nullptr)
-    p.lse[static_cast<long long>(it.s.start + tok) * p.Hq + head] =
-        (l != 0.f ? (m == -INFINITY ? 0.f : m) + fast_log2(l) : -INFINITY) * 0.6931471805599453f;
+  if (!it.whole) p.part_lse[part_row] = lse2;
+  else if (live && p.lse != nullptr) p.lse[static_cast<long long>(it.s.start + tok) * p.Hq + head] = lse2 * 0.6931471805599453f;
 }
 
 template <int D>
@@ -278,20 +301,20 @@ __device__ __forceinline__ void paged_mma_role(FaPagedTilesSmem<D>& s, const Abo
       phase ^= 1;
     }
   };
-  const int nmax = max(it.n[0], it.n[1]);
+  const int j0 = it.j0, nmax = it.j1;
   uint32_t slot_k = slot;
   if (!mbar_wait_warp(&s.kv_full[slot], phase, ctx, kRolePagedMma)) return;
   advance();
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    if ((i == 0 ? it.n[0] : it.n[1]) == 0) continue;
+    if ((i == 0 ? it.n[0] : it.n[1]) <= j0) continue;
     if (!mbar_wait_warp(&s.q_full[i], 0, ctx, kRolePagedMma)) return;
     tc_fence_after();
     issue_qk(i, slot_k);
     commit(&s.s_full[i]);
   }
   commit(&s.kv_empty[slot_k]);
-  for (int j = 0; j < nmax; ++j) {
+  for (int j = j0; j < nmax; ++j) {
     const uint32_t slot_v = slot;
     if (!mbar_wait_warp(&s.kv_full[slot], phase, ctx, kRolePagedMma)) return;
     advance();
@@ -302,9 +325,9 @@ __device__ __forceinline__ void paged_mma_role(FaPagedTilesSmem<D>& s, const Abo
     for (int i = 0; i < 2; ++i) {
       const int ni = i == 0 ? it.n[0] : it.n[1];
       if (j < ni) {
-        if (!mbar_wait_warp(&s.p_full[i], j & 1, ctx, kRolePagedMma)) return;
+        if (!mbar_wait_warp(&s.p_full[i], (j - j0) & 1, ctx, kRolePagedMma)) return;
         tc_fence_after();
-        issue_pv(i, slot_v, j > 0 ? 1u : 0u);
+        issue_pv(i, slot_v, j > j0 ? 1u : 0u);
         if (j == ni - 1) commit(&s.o_full[i]);
       }
       if (j + 1 < ni) {
@@ -343,7 +366,7 @@ __device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p,
 #pragma unroll
     for (int x = 0; x < 2; ++x) dst[k][x] = (ch >> 2) * (kTileN * 128) + row * 128 + ((2 * (ch & 3) + x) ^ (row & 7)) * 16;
   }
-  const int nmax = max(it.n[0], it.n[1]), len = it.s.len;
+  const int nmax = it.j1, len = it.s.len;
 
   // of key tile j, in lane g < 8: page and scales of keys 16 g .. + 15 (-1 and 0: none of the cache's, or behind the sequence)
   auto page_of = [&](int j) -> int {
@@ -403,11 +426,12 @@ __device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p,
       phase ^= 1;
     }
   };
-  int page = page_of(0);
+  int page = page_of(it.j0);
   float ks = scale_of(kv.k_scale, page), vs = scale_of(kv.v_scale, page);
   uint4 wk[kCopies], wv[kCopies];
-  fetch(k_base, kv.k_sp, kv.k_ss, 0, page, wk);
-  for (int j = 0; j < nmax; ++j) {
+  fetch(k_base, kv.k_sp, kv.k_ss, it.j0, page, wk);
+  for (int j = it.j0; j < nmax; ++j) {
+    const int at = (j - it.j0) % Smem::kMeta;
     const int next = page_of(j + 1);
     fetch(v_base, kv.v_sp, kv.v_ss, j, page, wv);
     // the tile's largest scales, and this warp's two halves relative to them
@@ -427,8 +451,8 @@ __device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p,
 
     if (!mbar_wait_warp(&s.kv_empty[slot], phase, ctx, kRolePagedProducer)) return;
     if (pw == 0 && lane == 0) {
-      s.meta[j % Smem::kMeta] = make_float4(k_ref, v_ref, __uint_as_float(gone), 0.f);
-      mbar_arrive(&s.meta_full[j % Smem::kMeta]);
+      s.meta[at] = make_float4(k_ref, v_ref, __uint_as_float(gone), 0.f);
+      mbar_arrive(&s.meta_full[at]);
     }
     store(slot, wk, k_alike, kr0, kr1);
     advance();
@@ -477,12 +501,14 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
   PagedItem it;
   {
     const KvView& kv = p.c;
+    const long long index = blockIdx.x / p.splits;  // of the item
+    const int split = static_cast<int>(blockIdx.x - index * p.splits);
     long long before = 0;
     if (kv.starts == nullptr && threadIdx.x == 0) {
       s.found = 0;
       s.found_at = 0;
     }
-    for (int b0 = kv.starts == nullptr ? kv.B : 0; b0 < kv.B && before <= blockIdx.x; b0 += kPagedTilesThreads) {
+    for (int b0 = kv.starts == nullptr ? kv.B : 0; b0 < kv.B && before <= index; b0 += kPagedTilesThreads) {
       const int b = b0 + threadIdx.x;
       const long long own = b < kv.B ? static_cast<long long>(paged_blocks_of(p, kv_seq(kv, b))) * kv.Hkv : 0;
       long long upto = own;
@@ -499,7 +525,7 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
         if (w < warp) upto += s.sums[w];
         before += s.sums[w];
       }
-      if (upto > blockIdx.x && upto - own <= blockIdx.x) {
+      if (upto > index && upto - own <= index) {
         s.found = b;
         s.found_at = upto - own;
       }
@@ -512,11 +538,12 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
     }
     __syncthreads();
     if (s.found < 0) {  // the grid is cut for the most items that so many rows can be
+      if (p.splits > 1 && split == 0 && threadIdx.x == 0) p.parts[index].count = 0;
       if (p.chained) grid_wait();
       return;
     }
     it.b = s.found;
-    const int in = static_cast<int>(blockIdx.x - s.found_at);
+    const int in = static_cast<int>(index - s.found_at);
     int rank = in / kv.Hkv;
     it.h = in - rank * kv.Hkv;
     if (kv.starts == nullptr) {
@@ -540,6 +567,26 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
         it.n[i] = tiles;
       }
     }
+    // its key tiles in equal parts, of four at least
+    const int most = max(it.n[0], it.n[1]), parts = min(p.splits, (most + 3) / 4);
+    if (p.splits > 1 && split == 0 && threadIdx.x == 0) {
+      PagedParts x;
+      x.count = parts;
+      x.h = it.h;
+      x.row0 = it.row0;
+      x.rows = it.rows;
+      x.start = it.s.start;
+      p.parts[index] = x;
+    }
+    if (split >= parts) {
+      if (p.chained) grid_wait();
+      return;
+    }
+    it.whole = parts == 1;
+    it.j0 = static_cast<int>(static_cast<long long>(most) * split / parts);
+    it.j1 = static_cast<int>(static_cast<long long>(most) * (split + 1) / parts);
+    it.n[0] = min(it.n[0], it.j1);
+    it.n[1] = min(it.n[1], it.j1);
   }
 
   if (warp == 8) {
@@ -578,6 +625,56 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Merges the parts of the items that are in any: a block has 32 rows of an item, a warp four of them, a lane D / 32 columns.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) fa_paged_tiles_combine_kernel(const __grid_constant__ FaPagedTilesParams p) {
+  grid_launch_dependents();
+  grid_wait();
+  constexpr int kCols = D / 32, kBlocks = kPagedBlockRows / 32;
+  const long long item = blockIdx.x / kBlocks;
+  const PagedParts x = p.parts[item];
+  if (x.count < 2) return;
+  const int lane = threadIdx.x & 31, r0 = static_cast<int>(blockIdx.x - item * kBlocks) * 32 + (threadIdx.x >> 5) * 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + k, row = x.row0 + r;
+    if (row >= x.rows) return;
+    auto at = [&](int part) -> long long { return (item * p.splits + part) * kPagedBlockRows + r; };
+    float top = lane < x.count ? p.part_lse[at(lane)] : -INFINITY;  // at most 32 parts
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = 0.f;
+    float acc[kCols] = {}, sum = 0.f;
+    for (int part = 0; part < x.count; ++part) {
+      const float lse = p.part_lse[at(part)];
+      if (lse == -INFINITY) continue;  // nothing was written
+      const float wt = fast_exp2(lse - top);
+      const float* src = p.part_o + at(part) * D + lane * kCols;
+      sum += wt;
+      if constexpr (kCols == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(src);
+        acc[0] = fmaf(wt, y.x, acc[0]);
+        acc[1] = fmaf(wt, y.y, acc[1]);
+        acc[2] = fmaf(wt, y.z, acc[2]);
+        acc[3] = fmaf(wt, y.w, acc[3]);
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(src);
+        acc[0] = fmaf(wt, y.x, acc[0]);
+        acc[1] = fmaf(wt, y.y, acc[1]);
+      }
+    }
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    const int tok = fast_div(row, p.by_group), head = x.h * p.group + row - tok * p.group;
+    T* dst = static_cast<T*>(p.o) + static_cast<long long>(x.start + tok) * p.o_st + head * p.o_sh + lane * kCols;
+    if constexpr (kCols == 4)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(Pack2<T>::pack(acc[0] * inv, acc[1] * inv), Pack2<T>::pack(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(dst) = Pack2<T>::pack(acc[0] * inv, acc[1] * inv);
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[static_cast<long long>(x.start + tok) * p.Hq + head] = (sum != 0.f ? top + fast_log2(sum) : -INFINITY) * 0.6931471805599453f;
   }
 }
 

@@ -49,11 +49,14 @@ __device__ __forceinline__ int append_exponent(float a) {
 }
 
 template <typename T>
-__device__ __forceinline__ void append_load8(const T* p, float* f) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void append_unpack8(const uint4& w, float* f) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) Pack2<T>::unpack(u[i], f[2 * i], f[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ void append_load8(const T* p, float* f) {
+  append_unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
 }
 template <typename T>
 __device__ __forceinline__ void append_store8(T* p, const float* f) {
@@ -111,27 +114,48 @@ __device__ __forceinline__ int append_seq_of(const KvAppendParams& p, int t) {
   return lo;
 }
 
+// Rotates the queries: a thread has eight pairs of kQueryRows rows, whose loads are on their way together.
+constexpr int kQueryRows = 2;
 template <typename T, int D>
 __device__ __forceinline__ void append_queries(const KvAppendParams& p) {
   constexpr int kPieces = D / 16;
-  const int item = (static_cast<int>(blockIdx.x) - p.cache_blocks) * kAppendThreads + static_cast<int>(threadIdx.x);
-  if (item >= p.q_items) return;
-  const int t = fast_div(item, p.by_q_row), r = item - t * static_cast<int>(p.by_q_row.d);
-  const int head = r / kPieces, piece = r % kPieces;
-  const KvSeq s = kv_seq(p.c, append_seq_of(p, t));
-  const int at = t - s.start, pos = s.pos0() + at;
-  if (at < 0 || at >= s.n) return;  // a row of no sequence
-  const T* src = static_cast<const T*>(p.q) + t * p.q_st + head * p.q_sh + piece * 8;
-  T* dst = static_cast<T*>(p.q_out) + t * p.qo_st + head * p.qo_sh + piece * 8;
-  float lo[8], hi[8];
-  append_load8(src, lo);
-  append_load8(src + D / 2, hi);
-  if (p.cos != nullptr) {
-    if (pos < 0 || pos >= p.rope_len) return;  // reported with the keys
-    append_rotate(lo, hi, p.cos + static_cast<long long>(pos) * (D / 2) + piece * 8, p.sin + static_cast<long long>(pos) * (D / 2) + piece * 8);
+  const int item0 = (static_cast<int>(blockIdx.x) - p.cache_blocks) * kAppendThreads * kQueryRows + static_cast<int>(threadIdx.x);
+  uint4 lo4[kQueryRows], hi4[kQueryRows];
+  int pos[kQueryRows];  // -1: nothing to do
+  T* dst[kQueryRows];
+#pragma unroll
+  for (int k = 0; k < kQueryRows; ++k) {
+    const int item = item0 + k * kAppendThreads;
+    pos[k] = -1;
+    if (item >= p.q_items) continue;
+    const int t = fast_div(item, p.by_q_row), r = item - t * static_cast<int>(p.by_q_row.d);
+    const int head = r / kPieces, piece = r % kPieces;
+    const T* src = static_cast<const T*>(p.q) + t * p.q_st + head * p.q_sh + piece * 8;
+    lo4[k] = *reinterpret_cast<const uint4*>(src);
+    hi4[k] = *reinterpret_cast<const uint4*>(src + D / 2);
+    dst[k] = static_cast<T*>(p.q_out) + t * p.qo_st + head * p.qo_sh + piece * 8;
+    const KvSeq s = kv_seq(p.c, append_seq_of(p, t));
+    const int at = t - s.start, x = s.pos0() + at;
+    // not a row of no sequence, nor one behind the tables (reported with the keys)
+    if (at >= 0 && at < s.n && (p.cos == nullptr || (x >= 0 && x < p.rope_len))) pos[k] = max(x, 0);
   }
-  append_store8(dst, lo);
-  append_store8(dst + D / 2, hi);
+  const int piece = item0 % kPieces;  // of every row of the thread
+#pragma unroll
+  for (int k = 0; k < kQueryRows; ++k) {
+    if (pos[k] < 0) continue;
+    if (p.cos != nullptr) {
+      float lo[8], hi[8];
+      append_unpack8<T>(lo4[k], lo);
+      append_unpack8<T>(hi4[k], hi);
+      const long long at = static_cast<long long>(pos[k]) * (D / 2) + piece * 8;
+      append_rotate(lo, hi, p.cos + at, p.sin + at);
+      append_store8(dst[k], lo);
+      append_store8(dst[k] + D / 2, hi);
+    } else {
+      *reinterpret_cast<uint4*>(dst[k]) = lo4[k];
+      *reinterpret_cast<uint4*>(dst[k] + D / 2) = hi4[k];
+    }
+  }
 }
 
 // GS threads own a unit.
@@ -365,7 +389,7 @@ extern "C" int hb_kv_append(const hb_kv_append_args* a) {
   const int64_t work = std::min<int64_t>(c.page_size, (static_cast<int64_t>(c.T) + c.B - 1) / c.B) * pieces;
   const int gs = work <= 64 ? 32 : work <= 128 ? 64 : kAppendThreads;
   p.cache_blocks = static_cast<int>((units + kAppendThreads / gs - 1) / (kAppendThreads / gs));
-  const int64_t grid = p.cache_blocks + (q_items + kAppendThreads - 1) / kAppendThreads;
+  const int64_t grid = p.cache_blocks + (q_items + kAppendThreads * kQueryRows - 1) / (kAppendThreads * kQueryRows);
   cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
   cudaError_t err;
   if (a->dtype == HB_BF16)
