@@ -133,8 +133,8 @@ static int launch_combine(const FaPagedParams& p, int rows, int blocks, cudaStre
   // parts of an item, where all items are alike
   const long long items = static_cast<long long>(p.c.B) * p.c.Hkv;
   const long long parts = (blocks + items - 1) / items + 1;
-  const int warps = parts <= 6 ? 1 : parts <= 24 ? 2 : parts <= 64 ? 4 : kPagedCombineWarps;  // to a row
-  const int rows_here = warps == kPagedCombineWarps ? 1 : warps == 4 ? 4 : 8;
+  // warps to a row, rows of a block.  us, B1 Hq32 Hkv8 D128 1000 keys (17 parts) with 2 x 8 | 4 x 2 | 8 x 1: 9.1 | 8.6 | 9.1, B3 Hq64 60011 keys (20) 54.4 | 54.0 | 56.5
+  const int warps = parts <= 6 ? 1 : parts <= 64 ? 4 : kPagedCombineWarps, rows_here = warps == 1 ? 8 : warps == 4 ? 2 : 1;
   HB_CUDA_CHECK(launch_dependent(fa_paged_combine_kernel<T, D>, blocks * (rows / rows_here), 32 * warps * rows_here, 0, stream, 0, p, rows, warps));
   return HB_OK;
 }

@@ -160,8 +160,7 @@ __device__ __forceinline__ void append_queries(const KvAppendParams& p) {
 
 // GS threads own a unit.
 template <typename T, int D, int GS>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
-  grid_launch_dependents();
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
   grid_wait();
   if (static_cast<int>(blockIdx.x) >= p.cache_blocks) {
     append_queries<T, D>(p);
@@ -314,6 +313,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     *reinterpret_cast<uint2*>(kp + kv_offset(place, c.k_ss) + D / 2 + piece * 8) = hi;
     *reinterpret_cast<uint4*>(vp + kv_offset(place, c.v_ss) + piece * 16) = val;
   }
+  grid_launch_dependents();  // let in at the start, they take the slots of blocks that have not begun: B4 prompts 37.3 -> 37.7 us
 }
 
 template <typename T, int D>

@@ -96,7 +96,7 @@ class Cache:
 
 
 def attend(q, cache, table, lens, starts=None, causal=True, scale=None):
-    """(O, LSE, and two error scales per output: sum p |v| / sum p, and sum of |v| of visible keys / sum exp(s - max)) in fp64."""
+    """(O, LSE, and three error scales: sum p |v| / sum p, keys x twice the largest |v| / sum exp(s - max), the scores' own) in fp64."""
     T, Hq, D = q.shape
     Hkv, size = cache.codes[0].shape[1], cache.codes[0].shape[2]
     scale = D ** -0.5 if scale is None else scale
@@ -127,10 +127,8 @@ def attend(q, cache, table, lens, starts=None, causal=True, scale=None):
                 out[row:row + n, hq] = torch.where(visible.any(-1)[:, None], (p @ vz) / safe, 0.0)
                 lse[row:row + n, hq] = (top + torch.log(total))[:, 0]
                 mean[row:row + n, hq] = (p @ vz.abs()) / safe
-                # every |v| times the largest magnitude stands for a code's: |code| v_ref <= 2 |v|'s own page's largest
                 spread[row:row + n, hq] = visible.double().sum(-1)[:, None] * v_ref * 2 / safe
                 if seen.any():
                     kabs = torch.where(seen[:, None], k, 0.0).abs()
-                    score_tol[row:row + n, hq] = scale * (rows.abs().amax(-1) * kabs.sum(-1).max() * 2.0 ** -17
-                                                          + (rows.abs() @ kabs.T).amax(-1) * D * 2.0 ** -24)
+                    score_tol[row:row + n, hq] = scale * (rows.abs() @ kabs.T).amax(-1) * D * 2.0 ** -23  # D sums in fp32, cut off or rounded
     return out, lse, mean, spread, score_tol

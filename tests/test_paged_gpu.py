@@ -150,9 +150,9 @@ def test_append_special_values(built_lib):
 def _close(got, lse, ref, dtype):
     out, want_lse, mean, spread, score = ref
     eps = torch.finfo(DT[dtype]).eps / 2
-    # P to 8 bits (2^-9), a score off by `score` moves its weight and the sum by as much (twice), 2^-18 of the largest P' in units of the
-    # largest value scale for every key, exponentials and sums 2^-20
-    tol = out.abs() * eps * 1.01 + (2.0 ** -9 + 2 * score[..., None] + 2.0 ** -19) * mean * (1 + 2.0 ** -6) + spread * 2.0 ** -18 + 1e-30
+    # P to fp16 (2^-12), a score off by `score` moves its weight and the sum by as much (twice), exponentials and sums 2^-20; what lies
+    # 2^-23 below the largest value scale may be lost for every key
+    tol = out.abs() * eps * 1.01 + (2.0 ** -12 + 2 * score[..., None] + 2.0 ** -19) * mean * (1 + 2.0 ** -6) + spread * 2.0 ** -22 + 1e-30
     bad = (got.double().cpu() - out).abs() > tol
     assert not bad.any(), ((got.double().cpu() - out).abs() / tol).max()
     assert not torch.isnan(got).any()
@@ -177,6 +177,13 @@ ATTENDS = [  # new, lens, page size, Hkv, group, D, dtype, layout, ragged call, 
     ([130, 3], [257, 3], 64, 1, 4, 64, "fp16", "bshd", True, True),
     ([60, 1], [200, 130], 32, 2, 2, 128, "fp16", "bhsd", True, False),
     ([260], [300], 64, 1, 2, 128, "bf16", "bhsd", True, True),
+    # many rows: keys of an item over several SMs, rows that see none of some part, tiles that end with the keys, pages of every size
+    ([128], [2000], 16, 1, 4, 128, "bf16", "bhsd", False, True),
+    ([300], [300], 128, 2, 3, 64, "fp16", "bshd", False, True),
+    ([256, 256], [1024, 1024], 64, 2, 1, 128, "fp16", "bhsd", False, True),
+    ([129] * 3, [640, 641, 129], 32, 1, 5, 64, "bf16", "bshd", False, False),
+    ([1, 400, 2, 90, 0, 33], [700, 900, 2, 1000, 50, 40], 64, 2, 4, 128, "bf16", "bshd", True, True),
+    ([70] * 40, [70 + 9 * b for b in range(40)], 32, 4, 2, 64, "fp16", "bhsd", False, True),
 ]
 
 
@@ -265,6 +272,24 @@ def test_what_the_device_finds_wrong(built_lib):
     after = P.Cache(pages)
     assert all(torch.equal(x, y) for x, y in zip(before.codes + before.scales, after.codes + after.scales))
     _clean()
+
+
+@pytest.mark.parametrize("new,group", ((100, 4), (200, 1)))
+def test_pages_that_are_not_there_for_many_rows(built_lib, new, group):
+    """The same with prompts: pages of nobody's and pages without scales within a tile of keys, in its last one, and a whole tile of them."""
+    from heddle_b200 import ops
+    g = _gen(41)
+    size, lens = 16, [700, 333]
+    pages, table = _cache(2, lens, size, 2, 128, "bhsd", g)
+    for block in (1, 20, *range(24, 32), 43):
+        table[0, block] = -1 if block % 2 else pages.k.shape[0] + block
+    scaleless = int(table[1, 5])
+    pages.k_scale[scaleless] = 0
+    q = torch.randn(2 * new, 2 * group, 128, device="cuda", generator=g).bfloat16()
+    out, lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    assert ops.cache_status() == 1 and ops.status_word() == 0
+    table[1, 5] = -1  # a page whose key scale is 0 is not there either
+    _close(out, lse, P.attend(q, P.Cache(pages), table.cpu(), lens), "bf16")
 
 
 def test_scales_of_any_size_and_peaked_rows(built_lib):
@@ -376,6 +401,58 @@ def test_results_repeat_and_do_not_depend_on_the_stream(built_lib):
     _clean()
     for out, lse in runs[1:]:
         assert torch.equal(out, runs[0][0]) and torch.equal(lse, runs[0][1])
+
+
+def test_prompts_captured_and_replayed(built_lib):
+    """A call of ragged prompts and single tokens is captured; lengths, starts and pages are others at its replays."""
+    from heddle_b200 import ops
+    g = _gen(43)
+    B, T, size = 4, 300, 32
+    pages, table = _cache(B, [900] * B, size, 2, 128, "bhsd", g)
+    q = torch.randn(T, 8, 128, device="cuda", generator=g).bfloat16()
+    lens, starts = _ints([900, 900, 900, 900]), _ints([0, 1, 250, 250, 300])
+    out = torch.full_like(q, 3.0)
+    call = lambda: ops.fa_paged(q, pages, table, lens, starts=starts, max_tokens=300, return_lse=True, out=out)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            _, lse = call()
+    torch.cuda.current_stream().wait_stream(side)
+    for new, n in (([1, 249, 0, 50], [900, 800, 0, 70]), ([100, 100, 99, 1], [100, 500, 129, 1]), ([1, 1, 1, 1], [33, 500, 128, 1]), ([0, 0, 300, 0], [5, 6, 640, 9])):
+        order = torch.randperm(B, generator=torch.Generator().manual_seed(sum(n))).tolist()
+        table.copy_(table[order].clone())
+        lens.copy_(_ints(n))
+        starts.copy_(torch.tensor([0] + new).cumsum(0).int())
+        out.fill_(3.0)
+        graph.replay()
+        _clean()
+        live = sum(new)
+        assert (out[live:] == 3.0).all()
+        _close(out[:live], lse[:live], P.attend(q[:live], P.Cache(pages), table.cpu(), n, starts.tolist()), "bf16")
+
+
+def test_calls_on_two_streams_at_once(built_lib):
+    from heddle_b200 import ops
+    g = _gen(47)
+    work = []
+    for B, n, lens in ((3, 1, [2000, 100, 900]), (2, 150, [600, 150]), (5, 1, [700] * 5), (1, 300, [1500])):
+        pages, table = _cache(B, lens, 64, 2, 128, "bhsd", g)
+        q = torch.randn(B * n, 8, 128, device="cuda", generator=g).bfloat16()
+        work.append((q, pages, table, _ints(lens)))
+    alone = [ops.fa_paged(*w, return_lse=True) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for _ in range(20):
+        for w, s in zip(work, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.fa_paged(*w, return_lse=True))
+    _clean()
+    for k, (out, lse) in enumerate(got):
+        assert torch.equal(out, alone[k % 4][0]) and torch.equal(lse, alone[k % 4][1])
 
 
 def test_sequences_share_a_prefix(built_lib):
