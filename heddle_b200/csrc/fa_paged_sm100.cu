@@ -39,75 +39,73 @@ static int64_t paged_most_rows(const hb_fa_paged_args* a) {
   if (c.starts == nullptr) return group * (c.T / c.B);
   return a->max_tokens > 0 ? group * std::min(a->max_tokens, c.T) : INT_MAX;
 }
-static int paged_tile_rows(const hb_fa_paged_args* a) { return paged_most_rows(a) <= 8 ? 8 : kPagedMaxRows; }
+// Which kernels a call takes and what they need; worked out from the arguments, which hold nothing that is on the device.
+struct PagedRoute {
+  bool rows_kernel, tiles_kernel;
+  int row_limit;              // the tiles kernel has the sequences of more query rows a KV head, the rows kernel the others
+  int tile_rows, blocks;      // rows kernel: rows of a row tile, blocks of the grid
+  int64_t items;              // tiles kernel: items, blocks of the grid for each
+  int splits;
+  uint64_t tiles_bytes, bytes;  // of the workspace: the tiles kernel's part, which comes first, and all
+};
 
-// As many blocks as the device holds, and no more than the list can fill: of tiles that the page table has room for.
-static int paged_blocks(const hb_fa_paged_args* a, int sm_count) {
-  const hb_kv_cache& c = a->cache;
-  const bool few = paged_tile_rows(a) == 8;
-  const int most = sm_count * (c.D == 128 ? (few ? paged_blocks_per_sm<128, 8> : paged_blocks_per_sm<128, 16>)
-                                          : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
-  const double row_tiles = (double)c.T * (a->Hq / c.Hkv) / paged_tile_rows(a) + c.B;
-  const double runs = row_tiles * c.Hkv * paged_places(paged_tiles(c.max_pages * c.page_size)) / kPagedWarps + 1;
-  return runs < most ? (int)runs : most;
+// Blocks for an item of the tiles kernel: as many as one round of blocks has place for, up to 16, each with three tiles at least of those that
+// the page table has room for.  More rounds of smaller blocks cost more than they even out, since a block's start and end take about as
+// long as five tiles.  us with 1 | 2 | 4 | 8 blocks an item: B1 Hq32 Hkv8, 128 rows, 4096 keys (16 items) 78.5 | 49.6 | 34.6 | 32.2; 512 rows (64 items)
+// 79 | 55 | 65 | 91; B1 Hq32 Hkv2, 128 rows, 20000 keys (16 items) 340 | 182 | 101 | 67; B4, 256 rows (128 items) 80 | 102 | 129 | 178.
+constexpr int kPagedMaxSplits = 16;
+static int paged_splits(int64_t items, double key_tiles, int sm_count) {
+  const int64_t round = items > 0 ? sm_count / items : 1;
+  return (int)std::max<int64_t>(1, std::min({round, (int64_t)(key_tiles / 3), (int64_t)kPagedMaxSplits}));
 }
 
-// Which kernels a call takes.  The tiles kernel has the sequences of more than paged_row_limit query rows a KV head, the rows kernel the
-// others; where the call says that there are none of the former (or all are), the other one is not launched.
 // The limit is where 32 keys cost the SMs as much either way, all sequences taken alike: in the rows kernel 375 cycles for every 16 rows,
-// dealt out evenly; in the tiles kernel 850 for up to 256, by rounds of whole blocks, or, where items are dealt out to several
-// blocks, divided by 0.6 of their number, which is what their starts and the merge leave of it.  us, rows kernel | tiles kernel, 4096 keys, Hq32 Hkv8: B1 64 rows (a KV head) 22
-// | 30, 256 rows 42 | 29; B4 48 rows 33 | 38, 128 rows 62 | 39; B16 32 rows 60 | 72, 48 rows 83 | 73; B64 32 rows 199 | 273, 48 rows 291 | 274.
-static int paged_splits_of(double items, double tiles, int sm_count);
-static double paged_most_tiles(const hb_fa_paged_args* a);
-static int paged_row_limit(const hb_fa_paged_args* a, int sm_count) {
-  const double items = (double)a->cache.B * a->cache.Hkv;
+// dealt out evenly; in the tiles kernel 850 for up to 256, by rounds of whole blocks, or, where items are dealt out to several blocks,
+// divided by 0.6 of their number, which is what their starts and the merge leave of it.  us, rows kernel | tiles kernel, Hq32 Hkv8, 4096
+// keys: B1 64 rows (a KV head) 22 | 25, 128 rows 28 | 26; B4 48 rows 32 | 32, 128 rows 62 | 33; B16 32 rows 59 | 73, 48 rows 83 | 73; B64 32 rows 199 | 277,
+// 48 rows 291 | 278.
+static int paged_row_limit(int64_t pairs, int64_t most_rows, double key_tiles, int sm_count) {
   int limit = kPagedMaxRows;
-  for (int tiles = 2; tiles <= 256; ++tiles) {
-    const double blocks = items * ((tiles * kPagedMaxRows + kPagedBlockRows - 1) / kPagedBlockRows);
-    const int splits = paged_splits_of(blocks, paged_most_tiles(a), sm_count);
-    const double rows_cost = items * tiles / sm_count * 375;
-    const double tiles_cost = 850 * (splits > 1 ? 1 / std::max(1.0, 0.6 * splits) : std::ceil(blocks / sm_count));
+  while (limit < most_rows && limit < 4096) {
+    const int tiles = limit / kPagedMaxRows + 1;
+    const int64_t blocks = pairs * ((tiles * kPagedMaxRows + kPagedBlockRows - 1) / kPagedBlockRows);
+    const int splits = paged_splits(blocks, key_tiles, sm_count);
+    const double rows_cost = (double)pairs * tiles / sm_count * 375;
+    const double tiles_cost = 850 * (splits > 1 ? 1 / std::max(1.0, 0.6 * splits) : (double)((blocks + sm_count - 1) / sm_count));
     if (rows_cost > tiles_cost) break;
-    limit = tiles * kPagedMaxRows;
+    limit += kPagedMaxRows;
   }
   return limit;
 }
-static bool paged_takes_tiles(const hb_fa_paged_args* a, int sm_count) { return paged_most_rows(a) > paged_row_limit(a, sm_count); }
-static bool paged_takes_rows(const hb_fa_paged_args* a, int sm_count) { return a->cache.starts != nullptr || !paged_takes_tiles(a, sm_count); }
 
-// Items of the tiles kernel: exactly, or where the device knows only, as many as so many rows can be.
-static int64_t paged_items(const hb_fa_paged_args* a, int sm_count) {
+static PagedRoute paged_route(const hb_fa_paged_args* a, int sm_count) {
   const hb_kv_cache& c = a->cache;
-  const int64_t group = a->Hq / c.Hkv, rows = group * c.T;
-  if (c.starts == nullptr) return static_cast<int64_t>(c.B) * c.Hkv * ((rows / c.B + kPagedBlockRows - 1) / kPagedBlockRows);
-  return c.Hkv * (rows / kPagedBlockRows + std::min<int64_t>(c.B, rows / (paged_row_limit(a, sm_count) + 1)));
-}
-// Blocks for an item: as many as one round of blocks has place for, up to 16, each with three tiles at least of those that the page
-// table has room for.  More rounds of smaller blocks cost more than they even out, since a block's start and end take about as long as
-// five tiles.  us with 1 | 2 | 4 | 8 blocks an item: B1 Hq32 Hkv8, 128 rows, 4096 keys (16 items) 78.5 | 49.6 | 34.6 | 32.2; 512 rows (64 items) 79 | 55
-// | 65 | 91; B1 Hq32 Hkv2, 128 rows, 20000 keys (16 items) 340 | 182 | 101 | 67; B4, 256 rows (128 items) 80 | 102 | 129 | 178.
-constexpr int kPagedMaxSplits = 16;
-static int paged_splits_of(double items, double tiles, int sm_count) {
-  return static_cast<int>(std::max(1.0, std::min({sm_count / std::max(items, 1.0), tiles / 3, (double)kPagedMaxSplits})));
-}
-static double paged_most_tiles(const hb_fa_paged_args* a) { return (double)a->cache.max_pages * a->cache.page_size / kTileN; }
-static int paged_splits(const hb_fa_paged_args* a, int sm_count) {
-  return paged_splits_of((double)paged_items(a, sm_count), paged_most_tiles(a), sm_count);
-}
-static uint64_t paged_tiles_workspace(const hb_fa_paged_args* a, int sm_count) {
-  if (!paged_takes_tiles(a, sm_count)) return 0;
-  const uint64_t splits = paged_splits(a, sm_count), items = paged_items(a, sm_count);
-  return splits > 1 ? items * (sizeof(PagedParts) + splits * kPagedBlockRows * (a->cache.D + 1) * sizeof(float)) : 0;
-}
-
-static uint64_t paged_workspace(const hb_fa_paged_args* a, int sm_count) {
-  uint64_t bytes = paged_tiles_workspace(a, sm_count);
-  if (paged_takes_rows(a, sm_count)) {
-    const uint64_t blocks = paged_blocks(a, sm_count), rows = paged_tile_rows(a);
-    bytes += 2 * blocks * rows * (a->cache.D + 1) * sizeof(float) + blocks * sizeof(PagedHead);
+  const int64_t group = a->Hq / c.Hkv, pairs = (int64_t)c.B * c.Hkv, all_rows = group * c.T, most_rows = paged_most_rows(a);
+  const double key_tiles = (double)c.max_pages * c.page_size / kTileN;
+  PagedRoute r = {};
+  r.row_limit = paged_row_limit(pairs, std::min(most_rows, all_rows), key_tiles, sm_count);
+  r.tiles_kernel = std::min(most_rows, all_rows) > r.row_limit;
+  r.rows_kernel = c.starts != nullptr || !r.tiles_kernel;
+  if (r.tiles_kernel) {
+    // exactly, or where the device knows only, as many as so many rows can be
+    if (c.starts == nullptr) r.items = pairs * ((all_rows / c.B + kPagedBlockRows - 1) / kPagedBlockRows);
+    else r.items = c.Hkv * (all_rows / kPagedBlockRows + std::min<int64_t>(c.B, all_rows / (r.row_limit + 1)));
+    r.splits = paged_splits(r.items, key_tiles, sm_count);
+    if (r.splits > 1) r.tiles_bytes = r.items * (sizeof(PagedParts) + (uint64_t)r.splits * kPagedBlockRows * (c.D + 1) * sizeof(float));
   }
-  return bytes;
+  r.bytes = r.tiles_bytes;
+  if (r.rows_kernel) {
+    r.tile_rows = most_rows <= 8 ? 8 : kPagedMaxRows;
+    // as many blocks as the device holds, and no more than the list can fill: of tiles that the page table has room for
+    const bool few = r.tile_rows == 8;
+    const int most = sm_count * (c.D == 128 ? (few ? paged_blocks_per_sm<128, 8> : paged_blocks_per_sm<128, 16>)
+                                            : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
+    const double row_tiles = (double)all_rows / r.tile_rows + c.B;
+    const double runs = row_tiles * c.Hkv * paged_places(paged_tiles(c.max_pages * c.page_size)) / kPagedWarps + 1;
+    r.blocks = runs < most ? (int)runs : most;
+    r.bytes += 2ull * r.blocks * r.tile_rows * (c.D + 1) * sizeof(float) + r.blocks * sizeof(PagedHead);
+  }
+  return r;
 }
 
 template <typename T, int D, int kRows>
@@ -185,7 +183,7 @@ extern "C" int hb_fa_paged_workspace(const hb_fa_paged_args* a, uint64_t* bytes)
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != HB_OK) return rc;
-  *bytes = paged_workspace(a, st->sm_count);
+  *bytes = paged_route(a, st->sm_count).bytes;
   return HB_OK;
 }
 
@@ -198,8 +196,9 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != HB_OK) return rc;
-  if (paged_items(a, st->sm_count) > 0x7fffffffll / (kPagedBlockRows / 32)) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
-  const uint64_t need = paged_workspace(a, st->sm_count);
+  const PagedRoute route = paged_route(a, st->sm_count);
+  if (route.items > 0x7fffffffll / (kPagedBlockRows / 32)) return set_error(HB_ERR_UNSUPPORTED, "hb_fa_paged: more than 2^31 blocks of query rows");
+  const uint64_t need = route.bytes;
   if (need > 0 && (workspace == nullptr || bytes < need))
     return set_error(HB_ERR_BAD_ARG, "hb_fa_paged: needs a workspace of %llu bytes, got %llu", (unsigned long long)need,
                      (unsigned long long)(workspace == nullptr ? 0 : bytes));
@@ -222,14 +221,12 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
     p.by_group = make_fast_div(p.group);
     p.scale_log2 = scale * 1.4426950408889634f;
   };
-  const int sm_count = st->sm_count;
-  const bool take_rows = paged_takes_rows(a, sm_count), take_tiles = paged_takes_tiles(a, sm_count);
   FaPagedParams p;
-  const int rows = paged_tile_rows(a), blocks = paged_blocks(a, sm_count);
-  if (take_rows) {
+  const int rows = route.tile_rows, blocks = route.blocks;
+  if (route.rows_kernel) {
     fill(p);
-    p.row_limit = take_tiles ? paged_row_limit(a, sm_count) : INT_MAX;
-    p.chained = take_tiles ? 1 : 0;
+    p.row_limit = route.tiles_kernel ? route.row_limit : INT_MAX;
+    p.chained = route.tiles_kernel ? 1 : 0;
     p.status = st->status_word;
     for (const bool keys : {true, false}) {
       // an axis of one page, head or token may carry any stride
@@ -242,20 +239,20 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
                              c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
       if (rc != HB_OK) return rc;
     }
-    p.heads = reinterpret_cast<PagedHead*>(static_cast<uint8_t*>(workspace) + paged_tiles_workspace(a, sm_count));
+    p.heads = reinterpret_cast<PagedHead*>(static_cast<uint8_t*>(workspace) + route.tiles_bytes);
     p.part_o = reinterpret_cast<float*>(p.heads + blocks);
     p.part_lse = p.part_o + 2ll * blocks * rows * c.D;
     rc = a->dtype == HB_BF16 ? launch_rows_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_rows_of<__half>(p, c.D, rows, blocks, stream);
     if (rc != HB_OK) return rc;
   }
   FaPagedTilesParams t;
-  const int64_t items = paged_items(a, sm_count);
-  if (take_tiles && items > 0) {
+  const int64_t items = route.items;
+  if (items > 0) {
     fill(t);
-    t.row_limit = paged_row_limit(a, sm_count);
-    t.chained = take_rows ? 1 : 0;
+    t.row_limit = route.row_limit;
+    t.chained = route.rows_kernel ? 1 : 0;
     t.status = st->status_word;
-    t.splits = paged_splits(a, sm_count);
+    t.splits = route.splits;
     t.parts = static_cast<PagedParts*>(workspace);
     t.part_o = t.splits > 1 ? reinterpret_cast<float*>(t.parts + items) : nullptr;
     t.part_lse = t.splits > 1 ? t.part_o + items * t.splits * kPagedBlockRows * c.D : nullptr;
@@ -264,11 +261,11 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
                              : launch_tiles_of<__half>(t, c.D, grid, st->smem_optin, stream);
     if (rc != HB_OK) return rc;
   }
-  if (take_rows) {
+  if (route.rows_kernel) {
     rc = a->dtype == HB_BF16 ? launch_combine_of<__nv_bfloat16>(p, c.D, rows, blocks, stream) : launch_combine_of<__half>(p, c.D, rows, blocks, stream);
     if (rc != HB_OK) return rc;
   }
-  if (!take_tiles || items == 0 || t.splits == 1) return HB_OK;
+  if (items == 0 || t.splits == 1) return HB_OK;
   const unsigned grid = static_cast<unsigned>(items * (kPagedBlockRows / 32));
   cudaError_t err;
   if (a->dtype == HB_BF16)
