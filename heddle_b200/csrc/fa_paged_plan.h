@@ -9,7 +9,9 @@
 
 namespace hb {
 
-constexpr int kPagedTile = 32;   // keys of a tile: what a warp works through at a time
+// Keys of a tile, what a warp works through at a time: 8 KB of codes either way.  us with 32 | 64 keys at D 64: B40 Hq12, one token, 900 to 1777 keys
+// 30.6 | 25.7; B1 Hq32 Hkv8, 20000 keys 21.3 | 15.0; B24 Hq32 Hkv8, four tokens 27.6 | 26.4; B128 Hq16, 100 keys (two tiles that meet) 19.0 | 22.0.
+HB_HD constexpr int paged_tile(int head_dim) { return head_dim == 128 ? 32 : 64; }
 constexpr int kPagedWarps = 4;   // of a block; they take the tiles of its run in turn
 
 // What a run pays for an item that it starts or goes on with, in tiles of the list: its queries, the meeting of the warps, the store
@@ -18,7 +20,7 @@ constexpr int kPagedWarps = 4;   // of a block; they take the tiles of its run i
 constexpr int kPagedItemCost = 6;
 
 // Key tiles of an item with `len` keys (an item without keys has a tile all the same: somebody has to write its rows).
-HB_HD int paged_tiles(int len) { return len <= 0 ? 1 : (len + kPagedTile - 1) / kPagedTile; }
+HB_HD int paged_tiles(int len, int tile = 32) { return len <= 0 ? 1 : static_cast<int>((static_cast<unsigned>(len) + tile - 1) / tile); }
 HB_HD int paged_places(int tiles) { return tiles + kPagedItemCost; }
 HB_HD int paged_row_tiles(int n, int group, int rows) {
   return static_cast<int>((static_cast<long long>(n) * group + rows - 1) / rows);

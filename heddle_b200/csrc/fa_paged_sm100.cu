@@ -101,7 +101,7 @@ static PagedRoute paged_route(const hb_fa_paged_args* a, int sm_count) {
     const int most = sm_count * (c.D == 128 ? (few ? paged_blocks_per_sm<128, 8> : paged_blocks_per_sm<128, 16>)
                                             : (few ? paged_blocks_per_sm<64, 8> : paged_blocks_per_sm<64, 16>));
     const double row_tiles = (double)all_rows / r.tile_rows + c.B;
-    const double runs = row_tiles * c.Hkv * paged_places(paged_tiles(c.max_pages * c.page_size)) / kPagedWarps + 1;
+    const double runs = row_tiles * c.Hkv * paged_places(paged_tiles(c.max_pages * c.page_size, paged_tile(c.D))) / kPagedWarps + 1;
     r.blocks = runs < most ? (int)runs : most;
     r.bytes += 2ull * r.blocks * r.tile_rows * (c.D + 1) * sizeof(float) + r.blocks * sizeof(PagedHead);
   }
@@ -234,7 +234,7 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
       const int64_t given[3] = {keys ? c.k_stride_s : c.v_stride_s, keys ? c.k_stride_h : c.v_stride_h, keys ? c.k_stride_p : c.v_stride_p};
       uint64_t strides[3];
       for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] > 1 ? (uint64_t)given[i] : (uint64_t)c.D;
-      const uint32_t box[4] = {(uint32_t)c.D, (uint32_t)std::min(c.page_size, kPagedTile), 1, 1};
+      const uint32_t box[4] = {(uint32_t)c.D, (uint32_t)std::min(c.page_size, paged_tile(c.D)), 1, 1};
       rc = encode_tensor_map(keys ? &p.tm_k : &p.tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box,
                              c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
       if (rc != HB_OK) return rc;

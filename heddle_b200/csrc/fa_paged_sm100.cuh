@@ -9,7 +9,7 @@
 // product by product (5.9 cycles of an SM for m16n8k32 against 2.0 for the fp16 product of half that depth).  So the codes are A and the
 // few query rows B: S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T, and nothing is padded beyond 8 rows.
 //
-// A warp works through tiles of 32 keys alone, from its own ring in shared memory, filled by TMA copies of a page's tokens (as 16-byte
+// A warp works through tiles of 32 keys (64 at D = 64) alone, from its own ring in shared memory, filled by TMA copies of a page's tokens (as 16-byte
 // asynchronous copies of each lane a tile's loads took 800 of its 3000 cycles).  Keys are numbered within a group of eight so that both readings of a tile (keys
 // along their rows, values across them) are free of bank conflicts; P goes from S^T's layout into B's by a transposing move,
 // and the pairs of value rows that a lane needs are put together by byte permutations.
@@ -19,7 +19,7 @@
 // workspace, and fa_paged_combine_kernel merges them.
 //
 // us of GPU time, both kernels (bytes the call cannot do without): B64 Hq32 Hkv8 D128, one token, 2000 to 4100 keys 71.0 (406 MB, 5.7 TB/s); B3 Hq64 Hkv8 D128,
-// 30 to 60 thousand keys 54.1 (5.1 TB/s); B24 Hq32 Hkv8 D128, four tokens, 1500 to 3000 keys 34.1 (3.4); B40 Hq12 Hkv12 D64 30.6 (2.7); B1, 1000 keys 8.8.
+// 30 to 60 thousand keys 54.1 (5.1 TB/s); B24 Hq32 Hkv8 D128, four tokens, 1500 to 3000 keys 34.1 (3.4); B40 Hq12 Hkv12 D64 25.7 (3.2); B1, 1000 keys 8.8.
 // About 10 us of each are the start (list, first pages), the meeting of the warps and the merge; the loop itself reads 6 TB/s.
 #pragma once
 
@@ -42,7 +42,7 @@ struct alignas(16) PagedHead {  // of an item in parts: where its parts lie (one
 };
 
 struct alignas(64) FaPagedParams {
-  CUtensorMap tm_k, tm_v;  // pages as [page][head][token][D], boxes of kPagedTile tokens (of a page, where it has fewer)
+  CUtensorMap tm_k, tm_v;  // pages as [page][head][token][D], boxes of a tile's tokens (of a page's, where it has fewer)
   KvView c;
   const void* q;
   void* o;
@@ -62,17 +62,18 @@ struct alignas(64) FaPagedParams {
 // Blocks an SM holds: what bounds a warp is the latency of its own instructions (four cycles and a half each with two warps to a
 // scheduler), so registers and the ring are cut to fit as many warps as do not spill.
 template <int D, int kRows>
-constexpr int paged_blocks_per_sm = D == 128 ? (kRows == 8 ? 3 : 2) : (kRows == 8 ? 4 : 3);
+constexpr int paged_blocks_per_sm = kRows == 8 || D == 64 ? 3 : 2;
 
 template <int D, int kRows>
 struct FaPagedSmem {
-  static constexpr int kTileBytes = kPagedTile * D;  // of keys, and of values
-  static constexpr int kStages = D == 128 ? (kRows == 8 ? 2 : 3) : 3;
+  static constexpr int kTile = paged_tile(D), kGroups = kTile / 16;
+  static constexpr int kTileBytes = kTile * D;  // of keys, and of values
+  static constexpr int kStages = paged_blocks_per_sm<D, kRows> == 3 ? 2 : 3;
   static constexpr int kFrags = kRows / 8 * (D / 16);  // accumulator tiles of O^T
   alignas(1024) uint8_t ring[kPagedWarps][kStages][2 * kTileBytes];
   float4 o[kPagedWarps / 2][kFrags][32];   // a warp's accumulators, as its lanes hold them ...
   float ml[kPagedWarps / 2][2][kRows];     // ... and its maxima and sums
-  alignas(16) float scales[kPagedWarps][kStages][4];  // keys, values of the tile's two halves; 0: a page that the cache does not have
+  alignas(16) float scales[kPagedWarps][kStages][2 * kGroups];  // of keys, of values of each 16 keys; 0: behind the sequence, or no page of the cache's
   uint64_t full[kPagedWarps][kStages];
   long long sums[kPagedWarps];
   long long found_at;
@@ -124,30 +125,31 @@ struct PagedCursor {
   int j;                 // key tile
 };
 // The sequence's part of the list: 0 where it has no rows, or too many for this kernel.
-__device__ __forceinline__ long long paged_list(const FaPagedParams& p, const KvSeq& s, int rows, int& tiles, int& row_tiles) {
-  tiles = paged_tiles(s.len);
+__device__ __forceinline__ long long paged_list(const FaPagedParams& p, const KvSeq& s, int rows, int tile, int& tiles, int& row_tiles) {
+  tiles = paged_tiles(s.len, tile);
   row_tiles = static_cast<long long>(s.n) * p.group <= p.row_limit ? paged_row_tiles(s.n, p.group, rows) : 0;
   return static_cast<long long>(paged_places(tiles)) * row_tiles * p.c.Hkv;
 }
-__device__ __forceinline__ void paged_enter(const FaPagedParams& p, PagedCursor& at, int rows) {
+__device__ __forceinline__ void paged_enter(const FaPagedParams& p, PagedCursor& at, int rows, int tile) {
   at.s = kv_seq(p.c, at.b);
-  (void)paged_list(p, at.s, rows, at.tiles, at.row_tiles);
+  (void)paged_list(p, at.s, rows, tile, at.tiles, at.row_tiles);
 }
 // To the first tile of the next item; only where the list has one.
-__device__ __forceinline__ void paged_next_item(const FaPagedParams& p, PagedCursor& at, int rows) {
+__device__ __forceinline__ void paged_next_item(const FaPagedParams& p, PagedCursor& at, int rows, int tile) {
   if (++at.rt < at.row_tiles) return;
   at.rt = 0;
   if (++at.h < p.c.Hkv) return;
   at.h = 0;
   do {
     if (++at.b >= p.c.B) return;
-    paged_enter(p, at, rows);
+    paged_enter(p, at, rows, tile);
   } while (at.row_tiles == 0);
 }
 
 template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)) fa_paged_rows_kernel(const __grid_constant__ FaPagedParams p) {
   using Smem = FaPagedSmem<D, kRows>;
+  constexpr int kTile = Smem::kTile, kGroups = Smem::kGroups;
   constexpr int kSteps = D / 16;  // products along head_dim
   constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
   constexpr int kN = kRows / 8;   // tiles of query rows
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   for (int b0 = 0; b0 < kv.B; b0 += kPagedThreads) {
     const int b = b0 + threadIdx.x;
     int tiles, row_tiles;
-    own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, tiles, row_tiles) : 0;
+    own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, kTile, tiles, row_tiles) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, upto, o);
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     for (int b0 = 0; b0 < kv.B && before <= begin; b0 += kPagedThreads) {
       const int b = b0 + threadIdx.x;
       int tiles, row_tiles;
-      own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, tiles, row_tiles) : 0;
+      own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, kTile, tiles, row_tiles) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, upto, o);
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
 
   PagedCursor seg;  // the segment's item and first tile
   seg.b = sm.found;
-  paged_enter(p, seg, kRows);
+  paged_enter(p, seg, kRows, kTile);
   long long t = begin;  // place of the segment's first tile in the list
   {
     const int places = paged_places(seg.tiles);
@@ -265,7 +267,12 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       }
     }
   };
-  fetch_q(seg);  // in front of the tiles, which the memory takes its time over
+  // A segment of one tile is its warp's alone, which stores the rows by itself: short items go to the warps in turn, and nobody waits.  us
+  // without | with: B128 Hq16 D128, 20 keys 18.6 | 11.4; B100 Hq32 Hkv8 D128, four tokens on themselves 18.4 | 9.6.
+  auto alone = [&](const PagedCursor& at, long long place) -> bool { return end - place == 1 || at.tiles - at.j == 1; };
+  int turn = 0;  // tiles of the run in front of the segment, modulo the warps
+  bool solo = alone(seg, t), mine = !solo || warp == 0;
+  if (mine) fetch_q(seg);  // in front of the tiles, which the memory takes its time over
 
   // ---- loads: the warp's next tile, while the ids of the pages of the one after are on their way
   PagedCursor ld = seg;
@@ -276,48 +283,42 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     while (ld.j >= ld.tiles && ld_left > kPagedItemCost) {
       ld.j -= ld.tiles;
       ld_left -= kPagedItemCost;
-      paged_next_item(p, ld, kRows);
+      paged_next_item(p, ld, kRows, kTile);
     }
     if (ld.j >= ld.tiles) ld_left = 0;
   };
-  // of the tile's halves, as the table has them (-1: behind the sequence); looked at when they are used: a warp stops where it looks
-  // at what has not come yet
-  auto pages = [&](int& first, int& second) {
-    const int tok = ld.j * kPagedTile;
-    const int* row = kv.table + ld.b * kv.table_stride + (tok >> kv.page_shift);
-    first = second = -1;
-    if (tok < ld.s.len) first = row[0];
-    if (kv.page_shift == 4 && tok + 16 < ld.s.len) second = row[1];
+  // the page of keys 16 (lane % kGroups) .. + 15 of the tile, as the table has it (-1: behind the sequence); looked at when it is used: a
+  // warp stops where it looks at what has not come yet
+  const int group0 = 16 * (lane & (kGroups - 1));
+  auto page_of = [&]() -> int {
+    const int tok = ld.j * kTile + group0;
+    return tok < ld.s.len ? kv.table[ld.b * kv.table_stride + (tok >> kv.page_shift)] : -1;
   };
-  int page0 = -1, page1 = -1;
+  int page = -1;
   skip(warp);
-  if (ld_left > 0) pages(page0, page1);
+  if (ld_left > 0) page = page_of();
   uint32_t ld_stage = 0;
   const int no_page = max(kv.num_pages, 1);  // the first coordinate outside of the cache: the copy writes zeros
+  const bool copies = lane < kGroups && (group0 & (min(1 << kv.page_shift, kTile) - 1)) == 0;  // the lane's keys begin a copy
   auto load = [&]() {                  // one tile, or nothing behind the run's end: a group of copies of scales either way
     if (ld_left > 0) {
-      const int tok = ld.j * kPagedTile, h = ld.h, len = ld.s.len, first = page0, second = page1;
+      const int tok = ld.j * kTile + group0, h = ld.h, len = ld.s.len;
+      const int id = static_cast<unsigned>(page) < static_cast<unsigned>(kv.num_pages) ? page : -1;
       skip(kPagedWarps);
-      if (ld_left > 0) pages(page0, page1);
-      const int a = static_cast<unsigned>(first) < static_cast<unsigned>(kv.num_pages) ? first : -1;
-      const int b = kv.page_shift > 4 ? a : static_cast<unsigned>(second) < static_cast<unsigned>(kv.num_pages) ? second : -1;
+      if (ld_left > 0) page = page_of();
       uint64_t* bar = &sm.full[warp][ld_stage];
-      uint8_t* dst = sm.ring[warp][ld_stage];
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, 2 * Smem::kTileBytes);
-        const int at = tok & ((1 << kv.page_shift) - 1);  // place of the tile's first key in its page
-        tma_load_4d(dst, &p.tm_k, bar, 0, at, h, a < 0 ? no_page : a);
-        tma_load_4d(dst + Smem::kTileBytes, &p.tm_v, bar, 0, at, h, a < 0 ? no_page : a);
-        if (kv.page_shift == 4) {
-          tma_load_4d(dst + 16 * D, &p.tm_k, bar, 0, 0, h, b < 0 ? no_page : b);
-          tma_load_4d(dst + Smem::kTileBytes + 16 * D, &p.tm_v, bar, 0, 0, h, b < 0 ? no_page : b);
-        }
-        if ((a < 0 && tok < len) || (b < 0 && tok + 16 < len)) kv_report(kv, HB_CACHE_BAD_PAGE);
+      if (lane == 0) mbar_arrive_expect_tx(bar, 2 * Smem::kTileBytes);
+      __syncwarp();
+      if (copies) {
+        uint8_t* dst = sm.ring[warp][ld_stage] + group0 * D;
+        const int at = tok & ((1 << kv.page_shift) - 1), coord = id < 0 ? no_page : id;
+        tma_load_4d(dst, &p.tm_k, bar, 0, at, h, coord);
+        tma_load_4d(dst + Smem::kTileBytes, &p.tm_v, bar, 0, at, h, coord);
       }
-      if (lane < 4) {
-        const int page = lane & 1 ? b : a;
-        const float* src = (lane & 2 ? kv.v_scale : kv.k_scale) + (page >= 0 ? static_cast<long long>(page) * kv.Hkv + h : 0);
-        cp_async4(smem_u32(&sm.scales[warp][ld_stage][lane]), src, page >= 0);
+      if (lane < 2 * kGroups) {
+        if (id < 0 && tok < len) kv_report(kv, HB_CACHE_BAD_PAGE);
+        const float* src = (lane >= kGroups ? kv.v_scale : kv.k_scale) + (id >= 0 ? static_cast<long long>(id) * kv.Hkv + h : 0);
+        cp_async4(smem_u32(&sm.scales[warp][ld_stage][lane]), src, id >= 0);
       }
       if (++ld_stage == Smem::kStages) ld_stage = 0;
     }
@@ -343,12 +344,38 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   // ---- segments
   uint32_t stage = 0, phase = 0;
   bool alive = true;  // until a wait gives up: then the block's barriers are all that is left to do
-  int turn = 0;  // tiles of the run in front of the segment, modulo the warps
   bool first = true;
   while (t < end) {
     const long long left = end - t;
     const int j0 = seg.j, j1 = left < seg.tiles - j0 ? j0 + static_cast<int>(left) : seg.tiles;
     const int rows = seg.s.n * p.group, row0 = seg.rt * kRows;
+    const bool whole = j0 == 0 && j1 == seg.tiles;
+    const int slot = 2 * run + (first ? 0 : 1);
+    const long long last = t + (seg.tiles - 1 - j0);  // place of the item's last tile
+    const bool more = last + kPagedItemCost + 1 < end;
+    const int next_turn = (turn + (j1 - j0)) & (kPagedWarps - 1);
+    if (warp == kPagedWarps - 1 && lane == 0 && j0 == 0 && !whole) {
+      PagedHead hd;
+      hd.last = paged_run_of(total, runs, last);
+      hd.slot = slot;
+      hd.h = seg.h;
+      hd.row0 = row0;
+      hd.start = seg.s.start;
+      hd.rows = rows;
+      p.heads[run] = hd;
+    }
+    if (!mine) {
+      if (!more) break;
+      paged_next_item(p, seg, kRows, kTile);
+      seg.j = 0;
+      t = last + kPagedItemCost + 1;
+      first = false;
+      turn = next_turn;
+      solo = alone(seg, t);
+      mine = !solo || warp == turn;
+      if (mine) fetch_q(seg);
+      continue;
+    }
 
     // B of S^T: the lane has columns 16 (c + 4 hh) .. + 15 of row g of each tile, scaled by 2^up, which takes the row's largest element
     // into [2^14, 2^15).  What it does with scores needs rows 2 c and 2 c + 1.
@@ -415,12 +442,19 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       __syncwarp();  // every lane's scales are there, and every lane is done with the tile before: its stage is free
       load();
       const uint32_t tile = smem_u32(sm.ring[warp][stage]);
-      const float4 scales = *reinterpret_cast<const float4*>(sm.scales[warp][stage]);
-
-      // scores of the 32 keys: row r of half t is key 16 t + (r ^ 4 (r & 1)); the lane has rows g and g + 8, columns 2 c and 2 c + 1
-      float x[kN][2][4];
+      float ks[kGroups], vs[kGroups];  // a group: 16 keys
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2 * kGroups; t += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(&sm.scales[warp][stage][t]);
+        const float z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) (t + e < kGroups ? ks[(t + e) % kGroups] : vs[(t + e) % kGroups]) = z[e];
+      }
+
+      // scores of the tile's keys: row r of group t is key 16 t + (r ^ 4 (r & 1)); the lane has rows g and g + 8, columns 2 c and 2 c + 1
+      float x[kN][kGroups][4];
+#pragma unroll
+      for (int t = 0; t < kGroups; ++t) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) x[n][t][0] = x[n][t][1] = x[n][t][2] = x[n][t][3] = 0.f;
 #pragma unroll
@@ -438,40 +472,50 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         }
       }
       // keys that a row does not see, or that are not there
-      if ((j + 1) * kPagedTile > least || scales.x == 0.f || scales.y == 0.f) {
+      bool there = true;
+      float v_top = 0.f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bool there = (t == 0 ? scales.x : scales.y) != 0.f;
+      for (int t = 0; t < kGroups; ++t) {
+        there = there && ks[t] != 0.f;
+        v_top = fmaxf(v_top, vs[t]);
+      }
+      if ((j + 1) * kTile > least || !there) {
+#pragma unroll
+        for (int t = 0; t < kGroups; ++t) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = j * kPagedTile + 16 * t + 8 * (e >> 1) + (g ^ ((g & 1) << 2));
+            const int key = j * kTile + 16 * t + 8 * (e >> 1) + (g ^ ((g & 1) << 2));
 #pragma unroll
             for (int n = 0; n < kN; ++n)
-              if (!there || key >= limit[n][e & 1]) x[n][t][e] = -INFINITY;
+              if (ks[t] == 0.f || key >= limit[n][e & 1]) x[n][t][e] = -INFINITY;
           }
         }
       }
       bool moved = false;
       float shrink_o = 1.f;
-      if (fmaxf(scales.z, scales.w) > v_ref) {  // powers of two; 0 at first, where O is 0
-        const float top = fmaxf(scales.z, scales.w);
-        shrink_o = v_ref / top;
-        v_ref = top;
-        to_ref = kPUnit / top;
+      if (v_top > v_ref) {  // powers of two; 0 at first, where O is 0
+        shrink_o = v_ref / v_top;
+        v_ref = v_top;
+        to_ref = kPUnit / v_top;
         moved = true;
       }
-      const __half2 pv[2] = {__float2half2_rn(scales.z * to_ref), __float2half2_rn(scales.w * to_ref)};  // at most kPUnit
+      __half2 pv[kGroups];  // at most kPUnit
+#pragma unroll
+      for (int t = 0; t < kGroups; ++t) pv[t] = __float2half2_rn(vs[t] * to_ref);
       float alpha[kN][2];
-      uint32_t pb[kN][2][2];  // P' as B of O^T
+      uint32_t pb[kN][kGroups][2];  // P' as B of O^T
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           // not 0 (a page without a scale, or less than fp32 holds): -inf has to stay it
-          float f0 = factor[n][e] * scales.x, f1 = factor[n][e] * scales.y;
-          f0 = f0 == 0.f ? 1.17549435e-38f : f0;
-          f1 = f1 == 0.f ? 1.17549435e-38f : f1;
-          float top = fmaxf(fmaxf(x[n][0][e], x[n][0][2 + e]) * f0, fmaxf(x[n][1][e], x[n][1][2 + e]) * f1);
+          float f[kGroups], top = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < kGroups; ++t) {
+            f[t] = factor[n][e] * ks[t];
+            f[t] = f[t] == 0.f ? 1.17549435e-38f : f[t];
+            top = fmaxf(top, fmaxf(x[n][t][e], x[n][t][2 + e]) * f[t]);
+          }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -480,14 +524,17 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           moved = moved || adopt;
           m[n][e] = adopt ? top : m[n][e];
           const float m_safe = m[n][e] == -INFINITY ? 0.f : m[n][e];
-          x[n][0][e] = fast_exp2(fmaf(x[n][0][e], f0, -m_safe));
-          x[n][0][2 + e] = fast_exp2(fmaf(x[n][0][2 + e], f0, -m_safe));
-          x[n][1][e] = fast_exp2(fmaf(x[n][1][e], f1, -m_safe));
-          x[n][1][2 + e] = fast_exp2(fmaf(x[n][1][2 + e], f1, -m_safe));
-          l[n][e] = fmaf(l[n][e], alpha[n][e], (x[n][0][e] + x[n][0][2 + e]) + (x[n][1][e] + x[n][1][2 + e]));
+          float sum = 0.f;
+#pragma unroll
+          for (int t = 0; t < kGroups; ++t) {
+            x[n][t][e] = fast_exp2(fmaf(x[n][t][e], f[t], -m_safe));
+            x[n][t][2 + e] = fast_exp2(fmaf(x[n][t][2 + e], f[t], -m_safe));
+            sum += x[n][t][e] + x[n][t][2 + e];
+          }
+          l[n][e] = fmaf(l[n][e], alpha[n][e], sum);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < kGroups; ++t) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const __half2 y = __hmul2(__floats2half2_rn(x[n][t][2 * h], x[n][t][2 * h + 1]), pv[t]);
@@ -508,10 +555,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           }
         }
       }
-      // O^T += V^T P'^T: of half t the lane has value rows 2 c, (2 c + 1) ^ 4 and those plus 8, columns D / 8 from D / 8 g on: rows g and
+      // O^T += V^T P'^T: of group t the lane has value rows 2 c, (2 c + 1) ^ 4 and those plus 8, columns D / 8 from D / 8 g on: rows g and
       // g + 8 of tile i are columns 2 i and 2 i + 1 of them
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < kGroups; ++t) {
         constexpr int kWords = D / 32;  // of 4 columns
         uint32_t vw[4][kWords];
 #pragma unroll
@@ -530,10 +577,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           }
         }
         // what a page holds behind the sequence is loaded with it; as numbers it may be anything, and 0 times it has to be 0
-        if ((j + 1) * kPagedTile > seg.s.len) {
+        if ((j + 1) * kTile > seg.s.len) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = j * kPagedTile + 16 * t + 8 * (i >> 1) + ((2 * c + (i & 1)) ^ ((i & 1) << 2));
+            const int key = j * kTile + 16 * t + 8 * (i >> 1) + ((2 * c + (i & 1)) ^ ((i & 1) << 2));
 #pragma unroll
             for (int w = 0; w < kWords; ++w) vw[i][w] = key < seg.s.len ? vw[i][w] : 0u;
           }
@@ -557,12 +604,13 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       }
     }
     PagedCursor next = seg;
-    const long long last = t + (seg.tiles - 1 - j0);  // place of the item's last tile
-    const bool more = last + kPagedItemCost + 1 < end;
+    bool next_solo = false, next_mine = false;
     if (more) {
-      paged_next_item(p, next, kRows);
+      paged_next_item(p, next, kRows, kTile);
       next.j = 0;
-      fetch_q(next);
+      next_solo = alone(next, last + kPagedItemCost + 1);
+      next_mine = !next_solo || warp == next_turn;
+      if (next_mine) fetch_q(next);
     }
 
     // ---- the warps' results meet: 2 and 3 hand theirs to 0 and 1, 1 to 0, which stores the rows
@@ -620,18 +668,18 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         }
       }
     };
-    const bool whole = j0 == 0 && j1 == seg.tiles;
-    const int slot = 2 * run + (first ? 0 : 1);
-    if (warp >= 2) give(warp - 2);
-    __syncthreads();
-    if (warp < 2) take(warp);
-    if (warp == 1) {
-      __syncwarp();
-      give(1);
+    if (!solo) {
+      if (warp >= 2) give(warp - 2);
+      __syncthreads();
+      if (warp < 2) take(warp);
+      if (warp == 1) {
+        __syncwarp();
+        give(1);
+      }
+      __syncthreads();
+      if (warp == 0) take(1);
     }
-    __syncthreads();
-    if (warp == 0) {
-      take(1);
+    if (solo || warp == 0) {
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
@@ -664,22 +712,14 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         }
       }
     }
-    if (warp == kPagedWarps - 1 && lane == 0 && j0 == 0 && !whole) {
-      PagedHead hd;
-      hd.last = paged_run_of(total, runs, last);
-      hd.slot = slot;
-      hd.h = seg.h;
-      hd.row0 = row0;
-      hd.start = seg.s.start;
-      hd.rows = rows;
-      p.heads[run] = hd;
-    }
-    __syncthreads();
-    turn = (turn + (j1 - j0)) & (kPagedWarps - 1);
+    if (!solo) __syncthreads();
+    turn = next_turn;
     if (!more) break;
     t = last + kPagedItemCost + 1;
     first = false;
     seg = next;
+    solo = next_solo;
+    mine = next_mine;
   }
   cp_async_wait<0>();
   if (!alive && lane == 0) {  // copies of this warp may be on their way into its ring: give them a while
