@@ -103,39 +103,58 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   const int limit = !live ? 0 : p.causal ? min(it.s.len, it.s.pos0() + tok + 1) : it.s.len;
   const int least = p.causal ? min(it.s.len, it.s.pos0() + fast_div(first, p.by_group) + 1) : it.s.len;
 
+  // Rows of q and o are read and written by D / 8 lanes each, so that a warp's access is whole rows, whoever owns them: by their owners a
+  // block's start took 8300 cycles for the queries and its end 3400 for the results.
+  constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+  const int piece = lane % kLanes;
+  auto tile_row = [&](int k) -> int { return (warp & 3) * 32 + k * kAtOnce + lane / kLanes; };
+  // of the lane's piece of that row, from the owner's place of the row; -1: not a row of the sequence
+  auto place = [&](int k, long long own) -> long long {
+    const long long at = __shfl_sync(0xffffffffu, own, k * kAtOnce + lane / kLanes);
+    return at < 0 ? -1 : at + 8 * piece;
+  };
+  auto staged = [&](int x, int e) -> uint4* {  // chunk e of row x: as the matrix instruction reads the queries
+    return reinterpret_cast<uint4*>(s.q[i] + (e >> 3) * (kTileM * 128) + x * 128 + ((e & 7) ^ (x & 7)) * 16);
+  };
+
   float factor;
-  {  // the row's queries in fp16: 2^up takes the largest element into [2^14, 2^15)
-    const T* src = static_cast<const T*>(p.q) + static_cast<long long>(it.s.start + tok) * p.q_st + head * p.q_sh;
-    uint4 w[D / 8];
-    float top = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int e = 0; e < D / 8; ++e) w[e] = live ? *reinterpret_cast<const uint4*>(src + 8 * e) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int e = 0; e < D / 8; ++e) {
-      const uint32_t u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a, b;
-        Pack2<T>::unpack(u[k], a, b);
-        top = max3(top, fabsf(a), fabsf(b));
-        finite = finite && fabsf(a) <= 3.402823466e38f && fabsf(b) <= 3.402823466e38f;
-      }
+  {  // the queries in fp16: 2^up takes a row's largest element into [2^14, 2^15)
+    // copied as they are, all on their way together, then scaled in place by their owner; in short loops, since what a block runs once
+    // it waits for the instructions of
+    const long long own = live ? (it.s.start + tok) * p.q_st + head * p.q_sh : -1;
+#pragma unroll 4
+    for (int k = 0; k < kLanes; ++k) {
+      const long long at = place(k, own);
+      cp_async16(smem_u32(staged(tile_row(k), piece)), static_cast<const T*>(p.q) + max(at, 0ll), at >= 0);
     }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncwarp();
+    uint32_t tops = 0u;  // without their signs, 16-bit numbers are in the order of their bits, infinities and NaN above all others
+#pragma unroll 4
+    for (int e = 0; e < D / 8; ++e) {
+      const uint4 w = *staged(r, e);
+      tops = __vimax3_u16x2(tops, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+      tops = __vimax3_u16x2(tops, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
+    }
+    float top, none;
+    Pack2<T>::unpack(max(tops & 0xffffu, tops >> 16), top, none);
+    const bool finite = top <= 3.402823466e38f;
     int up = 0;
-    if (top > 0.f && top <= 3.402823466e38f) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
+    if (top > 0.f && finite) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
     const float mul = __int_as_float((up + 127) << 23);
     factor = finite ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
-#pragma unroll
+#pragma unroll 4
     for (int e = 0; e < D / 8; ++e) {
-      uint32_t u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
+      const uint4 w = *staged(r, e);
+      uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float a, b;
         Pack2<T>::unpack(u[k], a, b);
         u[k] = Pack2<__half>::pack(a * mul, b * mul);
       }
-      *reinterpret_cast<uint4*>(s.q[i] + (e >> 3) * (kTileM * 128) + r * 128 + ((e & 7) ^ (r & 7)) * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+      *staged(r, e) = make_uint4(u[0], u[1], u[2], u[3]);
     }
     fence_proxy_async();
     __syncwarp();
@@ -239,9 +258,8 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   tc_fence_after();
   const float inv = l != 0.f ? v_unit * (1.f / 256.f) / l : 0.f;  // a row without keys is 0, one with a NaN is NaN
   const float lse2 = l != 0.f ? (m == -INFINITY ? 0.f : m) + fast_log2(l) : -INFINITY;
-  T* dst = static_cast<T*>(p.o) + static_cast<long long>(it.s.start + tok) * p.o_st + head * p.o_sh;
   float* part = p.part_o + (part_row - (r & 3)) * D;
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
     uint32_t o[32];
     __syncwarp();
@@ -250,12 +268,19 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     if (it.whole) {
       uint4 w[4];
       pack_row32<T>(o, inv, w);
-      if (live) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(dst + c * 32 + k * 8) = w[k];
-      }
+      for (int k = 0; k < 4; ++k) *staged(r, 4 * c + k) = w[k];  // the queries' products are complete
     } else {
       store_rows32_f32(part + c * 32, D, 4, o, inv);
+    }
+  }
+  if (it.whole) {
+    __syncwarp();
+    const long long own = live ? (it.s.start + tok) * p.o_st + head * p.o_sh : -1;
+#pragma unroll 4
+    for (int k = 0; k < kLanes; ++k) {
+      const long long at = place(k, own);
+      if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at) = *staged(tile_row(k), piece);
     }
   }
   if (!it.whole) p.part_lse[part_row] = lse2;
@@ -586,8 +611,8 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
       return;
     }
     it.whole = parts == 1;
-    it.j0 = static_cast<int>(static_cast<long long>(most) * split / parts);
-    it.j1 = static_cast<int>(static_cast<long long>(most) * (split + 1) / parts);
+    it.j0 = static_cast<int>(static_cast<unsigned>(most) * split / parts);  // most < 2^24, parts at most 16
+    it.j1 = static_cast<int>(static_cast<unsigned>(most) * (split + 1) / parts);
     it.n[0] = min(it.n[0], it.j1);
     it.n[1] = min(it.n[1], it.j1);
   }
