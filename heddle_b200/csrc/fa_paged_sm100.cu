@@ -250,6 +250,8 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
   if (items > 0) {
     fill(t);
     t.row_limit = route.row_limit;
+    t.by_hkv = make_fast_div(c.Hkv);
+    t.by_b = make_fast_div(c.B);
     t.chained = route.rows_kernel ? 1 : 0;
     t.status = st->status_word;
     t.splits = route.splits;

@@ -35,7 +35,7 @@ struct FaPagedTilesParams {
   int Hq, group, causal;
   int row_limit;  // sequences with no more query rows a KV head are the rows kernel's
   int chained;    // the rows kernel of the same call runs in front, and beside this one
-  FastDiv by_group;
+  FastDiv by_group, by_hkv, by_b;
   float scale_log2;
   uint32_t* status;
   int splits;       // blocks of the grid for an item: each has a part of its key tiles
@@ -84,6 +84,42 @@ __device__ __forceinline__ int paged_blocks_of(const FaPagedTilesParams& p, cons
   return rows > p.row_limit ? static_cast<int>((rows + kPagedBlockRows - 1) / kPagedBlockRows) : 0;
 }
 
+// Rows of q and o are read and written by D / 8 lanes each, whole rows an access, through the places of the queries in shared memory; by
+// their owners a block's start took 8300 cycles for the queries.
+template <int D>
+struct PagedRows {
+  static constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+  uint8_t* base;
+  int warp_row, sub, piece;
+  __device__ __forceinline__ PagedRows(FaPagedTilesSmem<D>& s, int i)
+      : base(s.q[i]), warp_row(threadIdx.x & (kTileM - 1) & ~31), sub((threadIdx.x & 31) / kLanes), piece(threadIdx.x % kLanes) {}
+  // chunk e of row x, where the matrix instruction reads the queries
+  __device__ __forceinline__ uint4* at(int x, int e) const {
+    return reinterpret_cast<uint4*>(base + (e >> 3) * (kTileM * 128) + x * 128 + ((e & 7) ^ (x & 7)) * 16);
+  }
+  __device__ __forceinline__ uint4* mine(int k) const { return at(warp_row + k * kAtOnce + sub, piece); }  // k < kLanes
+  // its place in global memory, from the owner's place of the row; -1: not a row of the sequence
+  __device__ __forceinline__ long long place(int k, long long own) const {
+    const long long row = __shfl_sync(0xffffffffu, own, k * kAtOnce + sub);
+    return row < 0 ? -1 : row + 8 * piece;
+  }
+};
+
+// The queries as they are; the softmax warps wait for them and scale them in place.
+template <typename T, int D>
+__device__ __forceinline__ void paged_copy_queries(const FaPagedTilesParams& p, FaPagedTilesSmem<D>& s, const PagedItem& it, int i) {
+  if ((i == 0 ? it.n[0] : it.n[1]) <= it.j0) return;
+  const PagedRows<D> rows(s, i);
+  const int row = it.row0 + kTileM * i + static_cast<int>(threadIdx.x & (kTileM - 1));
+  const int tok = fast_div(row, p.by_group);
+  const long long own = row < it.rows ? (it.s.start + tok) * p.q_st + (it.h * p.group + row - tok * p.group) * p.q_sh : -1;
+#pragma unroll 4
+  for (int k = 0; k < PagedRows<D>::kLanes; ++k) {
+    const long long at = rows.place(k, own);
+    cp_async16(smem_u32(rows.mine(k)), static_cast<const T*>(p.q) + max(at, 0ll), at >= 0);
+  }
+}
+
 template <typename T, int D>
 __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, FaPagedTilesSmem<D>& s, const AbortCtx& ctx, uint32_t tmem,
                                                    const PagedItem& it, int i) {
@@ -103,37 +139,15 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   const int limit = !live ? 0 : p.causal ? min(it.s.len, it.s.pos0() + tok + 1) : it.s.len;
   const int least = p.causal ? min(it.s.len, it.s.pos0() + fast_div(first, p.by_group) + 1) : it.s.len;
 
-  // Rows of q and o are read and written by D / 8 lanes each, so that a warp's access is whole rows, whoever owns them: by their owners a
-  // block's start took 8300 cycles for the queries and its end 3400 for the results.
-  constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
-  const int piece = lane % kLanes;
-  auto tile_row = [&](int k) -> int { return (warp & 3) * 32 + k * kAtOnce + lane / kLanes; };
-  // of the lane's piece of that row, from the owner's place of the row; -1: not a row of the sequence
-  auto place = [&](int k, long long own) -> long long {
-    const long long at = __shfl_sync(0xffffffffu, own, k * kAtOnce + lane / kLanes);
-    return at < 0 ? -1 : at + 8 * piece;
-  };
-  auto staged = [&](int x, int e) -> uint4* {  // chunk e of row x: as the matrix instruction reads the queries
-    return reinterpret_cast<uint4*>(s.q[i] + (e >> 3) * (kTileM * 128) + x * 128 + ((e & 7) ^ (x & 7)) * 16);
-  };
-
+  const PagedRows<D> rows(s, i);
   float factor;
   {  // the queries in fp16: 2^up takes a row's largest element into [2^14, 2^15)
-    // copied as they are, all on their way together, then scaled in place by their owner; in short loops, since what a block runs once
-    // it waits for the instructions of
-    const long long own = live ? (it.s.start + tok) * p.q_st + head * p.q_sh : -1;
-#pragma unroll 4
-    for (int k = 0; k < kLanes; ++k) {
-      const long long at = place(k, own);
-      cp_async16(smem_u32(staged(tile_row(k), piece)), static_cast<const T*>(p.q) + max(at, 0ll), at >= 0);
-    }
-    cp_async_commit();
     cp_async_wait<0>();
     __syncwarp();
     uint32_t tops = 0u;  // without their signs, 16-bit numbers are in the order of their bits, infinities and NaN above all others
-#pragma unroll 4
+#pragma unroll
     for (int e = 0; e < D / 8; ++e) {
-      const uint4 w = *staged(r, e);
+      const uint4 w = *rows.at(r, e);
       tops = __vimax3_u16x2(tops, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
       tops = __vimax3_u16x2(tops, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
     }
@@ -144,9 +158,9 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     if (top > 0.f && finite) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
     const float mul = __int_as_float((up + 127) << 23);
     factor = finite ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
-#pragma unroll 4
+#pragma unroll
     for (int e = 0; e < D / 8; ++e) {
-      const uint4 w = *staged(r, e);
+      const uint4 w = *rows.at(r, e);
       uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -154,7 +168,7 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
         Pack2<T>::unpack(u[k], a, b);
         u[k] = Pack2<__half>::pack(a * mul, b * mul);
       }
-      *staged(r, e) = make_uint4(u[0], u[1], u[2], u[3]);
+      *rows.at(r, e) = make_uint4(u[0], u[1], u[2], u[3]);
     }
     fence_proxy_async();
     __syncwarp();
@@ -269,7 +283,7 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
       uint4 w[4];
       pack_row32<T>(o, inv, w);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) *staged(r, 4 * c + k) = w[k];  // the queries' products are complete
+      for (int k = 0; k < 4; ++k) *rows.at(r, 4 * c + k) = w[k];  // the queries' products are complete
     } else {
       store_rows32_f32(part + c * 32, D, 4, o, inv);
     }
@@ -278,9 +292,9 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     __syncwarp();
     const long long own = live ? (it.s.start + tok) * p.o_st + head * p.o_sh : -1;
 #pragma unroll 4
-    for (int k = 0; k < kLanes; ++k) {
-      const long long at = place(k, own);
-      if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at) = *staged(tile_row(k), piece);
+    for (int k = 0; k < PagedRows<D>::kLanes; ++k) {
+      const long long at = rows.place(k, own);
+      if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at) = *rows.mine(k);
     }
   }
   if (!it.whole) p.part_lse[part_row] = lse2;
@@ -529,8 +543,8 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
   PagedItem it;
   {
     const KvView& kv = p.c;
-    const long long index = blockIdx.x / p.splits;  // of the item
-    const int split = static_cast<int>(blockIdx.x - index * p.splits);
+    const int index = p.splits == 1 ? blockIdx.x : blockIdx.x / p.splits;  // of the item
+    const int split = static_cast<int>(blockIdx.x) - index * p.splits;
     long long before = 0;
     if (kv.starts == nullptr && threadIdx.x == 0) {
       s.found = 0;
@@ -572,10 +586,10 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
     }
     it.b = s.found;
     const int in = static_cast<int>(index - s.found_at);
-    int rank = in / kv.Hkv;
+    int rank = fast_div(in, p.by_hkv);
     it.h = in - rank * kv.Hkv;
     if (kv.starts == nullptr) {
-      const int turn = rank / kv.B;
+      const int turn = fast_div(rank, p.by_b);
       it.b = rank - turn * kv.B;
       rank = turn;
     }
@@ -597,6 +611,7 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
     }
     // its key tiles in equal parts, of four at least
     const int most = max(it.n[0], it.n[1]), parts = min(p.splits, (most + 3) / 4);
+    it.whole = parts == 1;
     if (p.splits > 1 && split == 0 && threadIdx.x == 0) {
       PagedParts x;
       x.count = parts;
@@ -610,14 +625,16 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
       if (p.chained) grid_wait();
       return;
     }
-    it.whole = parts == 1;
-    it.j0 = static_cast<int>(static_cast<unsigned>(most) * split / parts);  // most < 2^24, parts at most 16
-    it.j1 = static_cast<int>(static_cast<unsigned>(most) * (split + 1) / parts);
+    it.j0 = it.whole ? 0 : static_cast<int>(static_cast<unsigned>(most) * split / parts);  // most < 2^24, parts at most 16
+    it.j1 = it.whole ? most : static_cast<int>(static_cast<unsigned>(most) * (split + 1) / parts);
     it.n[0] = min(it.n[0], it.j1);
     it.n[1] = min(it.n[1], it.j1);
   }
 
-  if (warp == 8) {
+  if (warp < 8) {
+    paged_copy_queries<T, D>(p, s, it, warp >> 2);
+    cp_async_commit();
+  } else if (warp == 8) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
   }
@@ -646,6 +663,7 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
     if (run) paged_producer_role<D>(p, s, ctx, it, warp - 12);
   }
   __syncwarp();
+  cp_async_wait<0>();
   tc_fence_before();
   if (p.chained) grid_wait();
   grid_launch_dependents();
