@@ -51,8 +51,8 @@ struct PagedRoute {
 
 // Blocks for an item of the tiles kernel: as many as one round of blocks has place for, up to 16, each with three tiles at least of those that
 // the page table has room for.  More rounds of smaller blocks cost more than they even out, since a block's start and end take about as
-// long as five tiles.  us with 1 | 2 | 4 | 8 blocks an item: B1 Hq32 Hkv8, 128 rows, 4096 keys (16 items) 78.5 | 49.6 | 34.6 | 32.2; 512 rows (64 items)
-// 79 | 55 | 65 | 91; B1 Hq32 Hkv2, 128 rows, 20000 keys (16 items) 340 | 182 | 101 | 67; B4, 256 rows (128 items) 80 | 102 | 129 | 178.
+// long as four tiles.  us with 1 | 2 | 4 | 8 blocks an item: B1 Hq32 Hkv8, 128 rows, 4096 keys (8 items) 71.4 | 42.8 | 28.1 | 22.8; 512 rows (16 items) 77 | 48 |
+// 32 | 31; B1 Hq32 Hkv2, 128 rows, 20000 keys (2 items) 328 | 169 | 91 | 55 (16: 39); B4, 256 rows, 2000 to 4096 keys (32 items) 77 | 49 | 36 | 44.
 constexpr int kPagedMaxSplits = 16;
 static int paged_splits(int64_t items, double key_tiles, int sm_count) {
   const int64_t round = items > 0 ? sm_count / items : 1;
@@ -61,9 +61,9 @@ static int paged_splits(int64_t items, double key_tiles, int sm_count) {
 
 // The limit is where 32 keys cost the SMs as much either way, all sequences taken alike: in the rows kernel 375 cycles for every 16 rows,
 // dealt out evenly; in the tiles kernel 850 for up to 256, by rounds of whole blocks, or, where items are dealt out to several blocks,
-// divided by 0.6 of their number, which is what their starts and the merge leave of it.  us, rows kernel | tiles kernel, Hq32 Hkv8, 4096
-// keys: B1 64 rows (a KV head) 22 | 25, 128 rows 28 | 26; B4 48 rows 32 | 32, 128 rows 62 | 33; B16 32 rows 59 | 73, 48 rows 83 | 73; B64 32 rows 199 | 277,
-// 48 rows 291 | 278.
+// divided by 0.6 of their number, which is what their starts and the merge leave of it.  us, rows kernel | tiles kernel, Hq32 Hkv8, 2000
+// to 4096 keys: B1 64 rows (a KV head) 19 | 23, 128 rows 26 | 23; B4 48 rows 31 | 31, 64 rows 35 | 31, 128 rows 61 | 32; B16 32 rows 51 | 75, 48 rows 70 | 74,
+// 64 rows 89 | 74; B64 32 rows 165 | 235, 48 rows 243 | 243.
 static int paged_row_limit(int64_t pairs, int64_t most_rows, double key_tiles, int sm_count) {
   int limit = kPagedMaxRows;
   while (limit < most_rows && limit < 4096) {
