@@ -140,3 +140,29 @@ def test_one_step_of_a_large_batch_captured(built_lib):
         want.append(k, v, table.cpu(), now)
         _close(out, None, P.attend(q, want, table.cpu(), now), "bf16")
     _clean()
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn(built_lib, seed):
+    """Batches of any mixture: items of one tile and of many in one run, sequences without rows or keys, heads in odd groups."""
+    import random
+
+    from heddle_b200 import ops
+    rng, g = random.Random(seed), _gen(151 + seed)
+    B, size, D = rng.choice((1, 3, 20, 150, 400)), rng.choice((16, 32, 64, 128)), rng.choice((64, 128))
+    Hkv, group, dtype = rng.choice((1, 2, 5)), rng.choice((1, 3, 4, 8, 9)), rng.choice(("bf16", "fp16"))
+    ragged, causal, layout = rng.random() < 0.6, rng.random() < 0.8, rng.choice(("bhsd", "bshd"))
+    most, longest = rng.choice((1, 1, 4, 60 if B <= 20 else 2)), rng.choice((8, 70, 200, 900 if B <= 20 else 130))
+    new = [rng.randint(0, most) for _ in range(B)] if ragged else [most] * B
+    lens = [n + rng.randint(0, longest) for n in new]
+    live = sum(new)
+    T = live + (2 if ragged else 0)
+    pages, table = _cache(B, lens, size, Hkv, D, layout, g)
+    q = (torch.randn(T, Hkv * group, D, device="cuda", generator=g) * 2).to(DT[dtype])
+    starts = torch.tensor([0] + new).cumsum(0).int().cuda() if ragged else None
+    out = torch.full_like(q, 7.0)
+    got, lse = ops.fa_paged(q, pages, table, _ints(lens), starts=starts, max_tokens=rng.choice((None, most)), causal=causal, return_lse=True, out=out)
+    _clean()
+    assert (out[live:] == 7.0).all()
+    ref = P.attend(q[:live], P.Cache(pages), table.cpu(), lens, None if starts is None else starts.tolist(), causal)
+    _close(got[:live], lse[:live], ref, dtype)
