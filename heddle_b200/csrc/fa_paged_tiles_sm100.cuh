@@ -98,10 +98,11 @@ struct PagedRows {
     return reinterpret_cast<uint4*>(base + (e >> 3) * (kTileM * 128) + x * 128 + ((e & 7) ^ (x & 7)) * 16);
   }
   __device__ __forceinline__ uint4* mine(int k) const { return at(warp_row + k * kAtOnce + sub, piece); }  // k < kLanes
-  // its place in global memory, from the owner's place of the row; -1: not a row of the sequence
+  // its place in global memory, from the owner's place of the row; kNone: not a row of the sequence (strides may be negative)
+  static constexpr long long kNone = -0x7fffffffffffffffll - 1;
   __device__ __forceinline__ long long place(int k, long long own) const {
     const long long row = __shfl_sync(0xffffffffu, own, k * kAtOnce + sub);
-    return row < 0 ? -1 : row + 8 * piece;
+    return row == kNone ? kNone : row + 8 * piece;
   }
 };
 
@@ -112,11 +113,12 @@ __device__ __forceinline__ void paged_copy_queries(const FaPagedTilesParams& p, 
   const PagedRows<D> rows(s, i);
   const int row = it.row0 + kTileM * i + static_cast<int>(threadIdx.x & (kTileM - 1));
   const int tok = fast_div(row, p.by_group);
-  const long long own = row < it.rows ? (it.s.start + tok) * p.q_st + (it.h * p.group + row - tok * p.group) * p.q_sh : -1;
+  const long long own = row < it.rows ? (it.s.start + tok) * p.q_st + (it.h * p.group + row - tok * p.group) * p.q_sh : PagedRows<D>::kNone;
 #pragma unroll 4
   for (int k = 0; k < PagedRows<D>::kLanes; ++k) {
     const long long at = rows.place(k, own);
-    cp_async16(smem_u32(rows.mine(k)), static_cast<const T*>(p.q) + max(at, 0ll), at >= 0);
+    const bool real = at != PagedRows<D>::kNone;
+    cp_async16(smem_u32(rows.mine(k)), static_cast<const T*>(p.q) + (real ? at : 0ll), real);
   }
 }
 
@@ -290,11 +292,11 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
   }
   if (it.whole) {
     __syncwarp();
-    const long long own = live ? (it.s.start + tok) * p.o_st + head * p.o_sh : -1;
+    const long long own = live ? (it.s.start + tok) * p.o_st + head * p.o_sh : PagedRows<D>::kNone;
 #pragma unroll 4
     for (int k = 0; k < PagedRows<D>::kLanes; ++k) {
       const long long at = rows.place(k, own);
-      if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at) = *rows.mine(k);
+      if (at != PagedRows<D>::kNone) *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at) = *rows.mine(k);
     }
   }
   if (!it.whole) p.part_lse[part_row] = lse2;

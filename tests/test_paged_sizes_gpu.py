@@ -166,3 +166,27 @@ def test_drawn(built_lib, seed):
     assert (out[live:] == 7.0).all()
     ref = P.attend(q[:live], P.Cache(pages), table.cpu(), lens, None if starts is None else starts.tolist(), causal)
     _close(got[:live], lse[:live], ref, dtype)
+
+
+@pytest.mark.parametrize("B,new", ((5, 1), (5, 4), (10, 70), (2, 256)))
+def test_rows_backwards(built_lib, B, new):
+    """Tokens and heads from the last to the first, through the C interface: strides may be negative."""
+    import ctypes as C
+
+    from heddle_b200 import _lib, ops
+    g = _gen(179)
+    Hkv, Hq, D = 8, 16, 128
+    T, lens = B * new, [300 + 17 * b for b in range(B)]
+    pages, table = _cache(B, lens, 32, Hkv, D, "bhsd", g)
+    q, seq_lens = torch.randn(T, Hq, D, device="cuda", generator=g).bfloat16(), _ints(lens)
+    want = ops.fa_paged(q, pages, table, seq_lens)
+    back, out = q.flip(0, 1).contiguous(), torch.zeros_like(q)
+    last = 2 * D * (T * Hq - 1)  # bytes in front of the last head of the last token
+    a = _lib.FaPagedArgs(ops._kv_cache("fa_paged", pages, table, seq_lens, None, q), back.data_ptr() + last, out.data_ptr() + last, None, -Hq * D, -D,
+                         -Hq * D, -D, Hq, 0, 1, D ** -0.5, ops._DTYPES[q.dtype], torch.cuda.current_stream().cuda_stream)
+    need = C.c_uint64(0)
+    _lib.check(_lib.load().hb_fa_paged_workspace(C.byref(a), C.byref(need)))
+    space = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    _lib.check(_lib.load().hb_fa_paged(C.byref(a), space.data_ptr(), need.value))
+    _clean()
+    assert torch.equal(out.flip(0, 1), want)
