@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   constexpr int kSteps = D / 16;  // products along head_dim
   constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
   constexpr int kN = kRows / 8;   // tiles of query rows
-  constexpr float kGrowth = 7.f, kPUnit = 256.f;
+  constexpr float kGrowth = 7.f, kPBits = 8.f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     const int least = p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(row0, p.by_group) + 1) : seg.s.len;
 
     float o[kN][kDims][4];
-    float m[kN][2], l[kN][2], v_ref = 0.f, to_ref = 0.f;  // O is in units of v_ref / kPUnit = 1 / to_ref
+    float m[kN][2], l[kN][2], v_ref = 0.f, to_ref = 0.f;  // O is in units of 2^-kPBits v_ref, l of 2^-kPBits; to_ref: 1 / v_ref
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
@@ -500,10 +500,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       if (v_top > v_ref) {  // powers of two; 0 at first, where O is 0
         shrink_o = v_ref / v_top;
         v_ref = v_top;
-        to_ref = kPUnit / v_top;
+        to_ref = 1.f / v_top;
         moved = true;
       }
-      __half2 pv[kGroups];  // at most kPUnit
+      __half2 pv[kGroups];  // at most 1
 #pragma unroll
       for (int t = 0; t < kGroups; ++t) pv[t] = __float2half2_rn(vs[t] * to_ref);
       float alpha[kN][2];
@@ -527,12 +527,13 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           alpha[n][e] = adopt ? fast_exp2(m[n][e] - top) : 1.f;
           moved = moved || adopt;
           m[n][e] = adopt ? top : m[n][e];
-          const float m_safe = m[n][e] == -INFINITY ? 0.f : m[n][e];
+          // the 2^kPBits go in here, in front of the rounding to fp16: its numbers below 2^-14 lose bits, those below 2^-25 are 0
+          const float off = kPBits - (m[n][e] == -INFINITY ? 0.f : m[n][e]);
           float sum = 0.f;
 #pragma unroll
           for (int t = 0; t < kGroups; ++t) {
-            x[n][t][e] = fast_exp2(fmaf(x[n][t][e], f[t], -m_safe));
-            x[n][t][2 + e] = fast_exp2(fmaf(x[n][t][2 + e], f[t], -m_safe));
+            x[n][t][e] = fast_exp2(fmaf(x[n][t][e], f[t], off));
+            x[n][t][2 + e] = fast_exp2(fmaf(x[n][t][2 + e], f[t], off));
             sum += x[n][t][e] + x[n][t][2 + e];
           }
           l[n][e] = fmaf(l[n][e], alpha[n][e], sum);
@@ -625,9 +626,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
         l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
         l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+        l[n][e] *= 1.f / 256.f;
       }
     }
-    const float unit = v_ref * (1.f / kPUnit);
+    const float unit = v_ref * (1.f / 256.f);
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
