@@ -13,7 +13,9 @@
 // asynchronous copies of each lane a tile's loads took 800 of its 3000 cycles).  Keys are numbered within a group of eight so that both readings of a tile (keys
 // along their rows, values across them) are free of bank conflicts; P goes from S^T's layout into B's by a transposing move,
 // and the pairs of value rows that a lane needs are put together by byte permutations.
-// A row's maximum is adopted when it grew by more than 2^7, as in fa_fwd: P' = 256 P vscale / v_ref stays within fp16.
+// What a row keeps the maximum of is score + log2 vscale, of the keys that it sees, so that P' = 2^8 P vscale, relative to that, is a number of fp16
+// whatever the scales are: it is 2^-33 of the row's largest product of weight and value scale at its finest.  The sum of the weights takes
+// the scales out again, by powers of two that fp32 holds.  A maximum is adopted when it grew by more than 2^7, as in fa_fwd.
 //
 // Work: the list of fa_paged_plan.h.  A run may start or end inside an item: such a segment leaves fp32 partial results in the
 // workspace, and fa_paged_combine_kernel merges them.
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   constexpr int kSteps = D / 16;  // products along head_dim
   constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
   constexpr int kN = kRows / 8;   // tiles of query rows
-  constexpr float kGrowth = 7.f, kPBits = 8.f;
+  constexpr float kGrowth = 7.f, kPBits = 8.f;  // P' is at most 2^15
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -385,7 +387,6 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     // into [2^14, 2^15).  What it does with scores needs rows 2 c and 2 c + 1.
     uint32_t qf[kN][kSteps][2];
     float factor[kN][2];
-    int limit[kN][2];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       float x[D / 64][16];
@@ -415,11 +416,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       const unsigned votes = __ballot_sync(0xffffffffu, finite);  // a row that holds an infinity or NaN is NaN
       const float f = ((votes >> (lane & ~3)) & 15u) == 15u ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
-        const int r = row0 + 8 * n + 2 * c + e;
-        limit[n][e] = r >= rows ? 0 : p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(r, p.by_group) + 1) : seg.s.len;
-      }
+      for (int e = 0; e < 2; ++e) factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
 #pragma unroll
       for (int hh = 0; hh < D / 64; ++hh) {
 #pragma unroll
@@ -430,7 +427,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     const int least = p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(row0, p.by_group) + 1) : seg.s.len;
 
     float o[kN][kDims][4];
-    float m[kN][2], l[kN][2], v_ref = 0.f, to_ref = 0.f;  // O is in units of 2^-kPBits v_ref, l of 2^-kPBits; to_ref: 1 / v_ref
+    // value scales are relative to `base`, the first tile's largest; m: the largest score + log2 vscale / base; O is in 2^(m - kPBits) base, l in
+    // 2^(m - kPBits)
+    float m[kN][2], l[kN][2];
+    int base = 0;  // bits; 0: no tile yet
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
@@ -476,36 +476,39 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         }
       }
       // keys that a row does not see, or that are not there
-      bool there = true;
-      float v_top = 0.f;
+      bool there = true, valued = true;
+      int v_top = 0;
 #pragma unroll
       for (int t = 0; t < kGroups; ++t) {
         there = there && ks[t] != 0.f;
-        v_top = fmaxf(v_top, vs[t]);
+        valued = valued && vs[t] != 0.f;
+        v_top = max(v_top, __float_as_int(vs[t]));
       }
+      if (base == 0) base = v_top;
       if ((j + 1) * kTile > least || !there) {
 #pragma unroll
-        for (int t = 0; t < kGroups; ++t) {
+        for (int n = 0; n < kN; ++n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = j * kTile + 16 * t + 8 * (e >> 1) + (g ^ ((g & 1) << 2));
+          for (int e = 0; e < 2; ++e) {
+            const int r = row0 + 8 * n + 2 * c + e;
+            const int limit = r >= rows ? 0 : p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(r, p.by_group) + 1) : seg.s.len;
+            const int key = j * kTile + (g ^ ((g & 1) << 2));
 #pragma unroll
-            for (int n = 0; n < kN; ++n)
-              if (ks[t] == 0.f || key >= limit[n][e & 1]) x[n][t][e] = -INFINITY;
+            for (int t = 0; t < kGroups; ++t) {
+              if (ks[t] == 0.f || key + 16 * t >= limit) x[n][t][e] = -INFINITY;
+              if (ks[t] == 0.f || key + 16 * t + 8 >= limit) x[n][t][2 + e] = -INFINITY;
+            }
           }
         }
       }
       bool moved = false;
-      float shrink_o = 1.f;
-      if (v_top > v_ref) {  // powers of two; 0 at first, where O is 0
-        shrink_o = v_ref / v_top;
-        v_ref = v_top;
-        to_ref = 1.f / v_top;
-        moved = true;
-      }
-      __half2 pv[kGroups];  // at most 1
+      float v_log[kGroups], v_inv[kGroups];  // log2 vscale / base and its inverse; where the scale is 0, as if it were base, and the values are 0
 #pragma unroll
-      for (int t = 0; t < kGroups; ++t) pv[t] = __float2half2_rn(vs[t] * to_ref);
+      for (int t = 0; t < kGroups; ++t) {
+        const int to = vs[t] != 0.f ? min(max(__float_as_int(vs[t]) - base, -(126 << 23)), 126 << 23) : 0;
+        v_log[t] = static_cast<float>(to >> 23);
+        v_inv[t] = __int_as_float((127 << 23) - to);
+      }
       float alpha[kN][2];
       uint32_t pb[kN][kGroups][2];  // P' as B of O^T
 #pragma unroll
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           for (int t = 0; t < kGroups; ++t) {
             f[t] = factor[n][e] * ks[t];
             f[t] = f[t] == 0.f ? 1.17549435e-38f : f[t];
-            top = fmaxf(top, fmaxf(x[n][t][e], x[n][t][2 + e]) * f[t]);
+            top = fmaxf(top, fmaf(fmaxf(x[n][t][e], x[n][t][2 + e]), f[t], v_log[t]));
           }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
@@ -532,9 +535,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           float sum = 0.f;
 #pragma unroll
           for (int t = 0; t < kGroups; ++t) {
-            x[n][t][e] = fast_exp2(fmaf(x[n][t][e], f[t], off));
-            x[n][t][2 + e] = fast_exp2(fmaf(x[n][t][2 + e], f[t], off));
-            sum += x[n][t][e] + x[n][t][2 + e];
+            const float off_t = off + v_log[t];
+            x[n][t][e] = fast_exp2(fmaf(x[n][t][e], f[t], off_t));
+            x[n][t][2 + e] = fast_exp2(fmaf(x[n][t][2 + e], f[t], off_t));
+            sum = fmaf(x[n][t][e] + x[n][t][2 + e], v_inv[t], sum);
           }
           l[n][e] = fmaf(l[n][e], alpha[n][e], sum);
         }
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         for (int t = 0; t < kGroups; ++t) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const __half2 y = __hmul2(__floats2half2_rn(x[n][t][2 * h], x[n][t][2 * h + 1]), pv[t]);
+            const __half2 y = __floats2half2_rn(x[n][t][2 * h], x[n][t][2 * h + 1]);
             pb[n][t][h] = movmatrix(*reinterpret_cast<const uint32_t*>(&y));
           }
         }
@@ -550,7 +554,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-          const float f0 = alpha[n][0] * shrink_o, f1 = alpha[n][1] * shrink_o;
+          const float f0 = alpha[n][0], f1 = alpha[n][1];
 #pragma unroll
           for (int i = 0; i < kDims; ++i) {
             o[n][i][0] *= f0;
@@ -582,12 +586,12 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           }
         }
         // what a page holds behind the sequence is loaded with it; as numbers it may be anything, and 0 times it has to be 0
-        if ((j + 1) * kTile > seg.s.len) {
+        if ((j + 1) * kTile > seg.s.len || !valued) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = j * kTile + 16 * t + 8 * (i >> 1) + ((2 * c + (i & 1)) ^ ((i & 1) << 2));
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) vw[i][w] = key < seg.s.len ? vw[i][w] : 0u;
+            for (int w = 0; w < kWords; ++w) vw[i][w] = key < seg.s.len && sm.scales[warp][stage][kGroups + t] != 0.f ? vw[i][w] : 0u;
           }
         }
 #pragma unroll
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
         l[n][e] *= 1.f / 256.f;
       }
     }
-    const float unit = v_ref * (1.f / 256.f);
+    const float unit = __int_as_float(base) * (1.f / 256.f);
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll

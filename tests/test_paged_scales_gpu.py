@@ -8,6 +8,9 @@ from test_paged_gpu import DT, _cache, _clean, _gen, _ints
 
 pytestmark = pytest.mark.gpu
 
+FEW = dict(B=5, Hkv=2, group=2)    # the rows kernel, whatever the number of tokens up to 64
+
+
 def _reference(q, pages, table, lens, new, causal, floor):
     """(O, LSE, tolerances of both) in fp64.  ``floor``: P is kept as a multiple of 2^-24 of what O is held in, so that every key's weight may be
     off by 2^-25 of that; O is held in 2^-8 of a unit which is at most 2^9 times the largest product of a visible key's weight and its
@@ -61,6 +64,104 @@ def _check(got, got_lse, ref):
     empty = lse == -math.inf
     assert torch.equal(got_lse == -math.inf, empty)
     assert ((got_lse.double() - lse).abs() <= lse_tol)[~empty].all()
+
+
+def _blocks(pages, table, which, exponents):
+    """Scales of the sequences' blocks: 2^exponents(block, blocks)."""
+    scale = (pages.k_scale, pages.v_scale)[which]
+    for block in range(table.shape[1]):
+        scale[table[:, block].long()] = 2.0 ** exponents(block, table.shape[1])
+
+
+def _setting(kind, spread, pages, table, q, g):
+    """Scales, keys and queries in which a page far above the others must not decide the result."""
+    later = lambda block, blocks: -6 if block >= (blocks + 1) // 2 else -6 - spread  # noqa: E731
+    if kind == "values behind the causal limit":
+        _blocks(pages, table, 1, later)
+    elif kind == "keys behind the causal limit":
+        _blocks(pages, table, 0, later)
+        q.mul_(2.0 ** min(spread, 12))  # fp16 holds that; scores of some size where the small keys alone are seen
+    elif kind == "keys that a query has no part in":  # every third page, in the upper half of head_dim, where the queries are 0
+        D = q.shape[2]
+        _blocks(pages, table, 0, lambda block, blocks: -6 + spread if block % 3 == 1 else -6)
+        for block in range(1, table.shape[1], 3):
+            pages.k.view(torch.uint8)[table[:, block].long()[:, None, None], :, :, :D // 2] = 0
+        q[..., D // 2:] = 0
+    elif kind == "values seen with a low score":
+        _blocks(pages, table, 0, lambda block, blocks: -6)
+        _blocks(pages, table, 1, lambda block, blocks: -6 + spread if block % 4 == 2 else -6)
+        one = torch.tensor([1.0, -448.0], device="cuda").to(torch.float8_e4m3fn).view(torch.uint8)
+        pages.k.view(torch.uint8)[..., 0] = one[0]
+        for block in range(2, table.shape[1], 4):  # weights of about 2^-spread
+            pages.k.view(torch.uint8)[table[:, block].long(), ..., 0] = one[1]
+        q[..., 0] = spread * math.log(2) * q.shape[2] ** 0.5 * 64 / 448
+    else:  # steps that add up, and any
+        if kind == "values in steps":
+            _blocks(pages, table, 1, lambda block, blocks: -40 + (block * spread) // blocks)
+        else:
+            pages.v_scale.copy_(torch.exp2(torch.randint(-spread, 1, pages.v_scale.shape, device="cuda", generator=g).float()))
+            pages.k_scale.copy_(torch.exp2(torch.randint(-spread // 2 - 3, -3, pages.k_scale.shape, device="cuda", generator=g).float()))
+
+
+KINDS = ("values behind the causal limit", "keys behind the causal limit", "keys that a query has no part in", "values seen with a low score",
+         "values in steps", "any")
+CALLS = [  # form, new, length, page size, D, dtype, layout
+    (FEW, 4, 18, 16, 128, "bf16", "bhsd"),
+    (FEW, 3, 200, 16, 64, "fp16", "bshd"),
+    (FEW, 1, 1000, 32, 128, "fp16", "bhsd"),
+    (FEW, 60, 130, 16, 64, "bf16", "bhsd"),
+]
+
+
+@pytest.mark.parametrize("spread", (9, 16, 25, 40))
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form,new,length,size,D,dtype,layout", CALLS)
+def test_scales_far_apart(built_lib, form, new, length, size, D, dtype, layout, kind, spread):
+    from heddle_b200 import ops
+    g = _gen(191)
+    B, Hkv, group = form["B"], form["Hkv"], form["group"]
+    lens = [length - b for b in range(B)]
+    lens = [max(n, new) for n in lens]
+    pages, table = _cache(B, lens, size, Hkv, D, layout, g)
+    q = (torch.randn(B * new, Hkv * group, D, device="cuda", generator=g)).to(DT[dtype])
+    heads_first = pages if layout == "bhsd" else pages._replace(k=pages.k.transpose(1, 2), v=pages.v.transpose(1, 2))
+    _setting(kind, spread, heads_first, table, q, g)
+    out, lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    _clean()
+    _check(out, lse, _reference(q, pages, table, lens, [new] * B, True, 24))
+
+
+@pytest.mark.parametrize("form,new,length,size,D", ((FEW, 4, 100, 16, 128), (FEW, 2, 300, 32, 64)))
+def test_scales_far_apart_among_pages_that_are_not_there(built_lib, form, new, length, size, D):
+    """The same with pages of nobody's, value scales of 0, and sequences without keys; then with a NaN key and a NaN query."""
+    from heddle_b200 import ops
+    g = _gen(193)
+    B, Hkv, group = form["B"], form["Hkv"], form["group"]
+    lens = [length - 3 * b for b in range(B)]
+    lens[1] = 0
+    pages, table = _cache(B, lens, size, Hkv, D, "bhsd", g)
+    q = torch.randn(B * new, Hkv * group, D, device="cuda", generator=g).bfloat16()
+    _setting("any", 40, pages, table, q, g)
+    for block in (1, 2, 5):
+        table[0, block] = -1
+        pages.v_scale[table[2, block].long()] = 0
+    out, lse = ops.fa_paged(q, pages, table, _ints(lens), causal=False, return_lse=True)
+    assert ops.cache_status() == 3 and ops.status_word() == 0  # a page outside of the cache, a sequence shorter than its rows
+    live = torch.ones(B * new, dtype=torch.bool, device="cuda")
+    live[new:2 * new] = False
+    keep = [b for b in range(B) if b != 1]
+    ref = _reference(q[live], pages, table[keep], [lens[b] for b in keep], [new] * (B - 1), False, 24)
+    _check(out[live], lse[live], ref)
+    assert (out[~live] == 0).all() and (lse[~live] == -math.inf).all()
+    pages.k.view(torch.uint8)[table[2, 3].long(), Hkv - 1, size - 1] = 0x7F  # as kv_append stores a token with a NaN
+    q[0, 0, 5] = math.nan
+    sick = torch.zeros(B * new, Hkv * group, dtype=torch.bool, device="cuda")
+    sick[0, 0] = True
+    sick[2 * new:3 * new, (Hkv - 1) * group:] = True
+    again, again_lse = ops.fa_paged(q, pages, table, _ints(lens), causal=False, return_lse=True)
+    assert ops.cache_status() == 3 and ops.status_word() == 0
+    assert torch.isnan(again[sick]).all() and torch.isnan(again_lse[sick]).all()
+    assert torch.equal(again[~sick], out[~sick]) and torch.equal(again_lse[~sick], lse[~sick])
 
 
 @pytest.mark.parametrize("D,dtype", ((64, "bf16"), (64, "fp16"), (128, "bf16"), (128, "fp16")))
