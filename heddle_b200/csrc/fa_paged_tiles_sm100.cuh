@@ -6,12 +6,13 @@
 //     operands that tcgen05.mma reads (128-byte swizzle; keys K-major, values MN-major), each tile once for 256 rows.  Two
 //     e4m3 products of a query's and a weight's parts would need no conversion, and twice the products and a split of every weight;
 //   - the scales of a tile's pages are taken relative to the tile's largest, powers of two that fp16 holds beside the code; where all
-//     are alike, nearly always, nothing is multiplied.  The largest goes into the factor of the scores and the unit of P';
+//     are alike, nearly always, nothing is multiplied.  The largest goes into the factor of the scores and into the weights P'.  Where
+//     scales of a tile are more than 2^8 apart its codes stay as they are, and the softmax has the scales of every 16 keys;
 //   - queries are scaled into fp16 by a power of two for each row, by the thread that owns the row.
 // An item's key tiles are dealt out to several blocks where items are few, or do not fill the SMs evenly (paged_splits); their fp32 partial
 // results meet in fa_paged_tiles_combine_kernel.
-// A row's maximum is adopted when it grew by more than 2^7, and O's unit when a tile has a larger value scale: P' = 256 P
-// (scale / unit).  O is rescaled by the row's own thread, as in fa_split.
+// A row's maximum is that of score + log2 value scale, adopted when it grew by more than 2^7 (fa_paged_sm100.cuh).  O is rescaled by the row's
+// own thread, as in fa_split.
 //
 // us of GPU time: B2 Hq32 Hkv8 D128, 2048 queries behind 6144 505 (0.94 PFLOP/s; tensor pipe and MUFU 48 % each, at the power cap, as fa_fwd); B4 Hq16
 // Hkv16 D64, prompts of 1024 33.6; B16 Hq28 Hkv4 D128, 1 to 400 queries behind 750 to 1500 104.3.  The short ones pay for starts and ends of blocks.
@@ -59,7 +60,8 @@ struct FaPagedTilesSmem {
   // K(j + kMeta) takes the ring's place of tile 2 (j + kMeta) - kStages of K(0) V(0) K(1) V(1) ..: where that is V(j) or later, P(j) was
   // there, and so meta(j) read
   static_assert(2 * kMeta - kStages >= 1, "a tile's scales are overwritten only when its softmax is done");
-  float4 meta[kMeta];  // of key tile j at j % kMeta: largest key scale, largest value scale, bits of groups of 16 keys that are not there
+  float4 meta[kMeta];  // of key tile j at j % kMeta: largest key scale, largest value scale, bits of groups of 16 keys that are not there, 1: ...
+  float2 group[kMeta][kTileN / 16];  // ... the codes are as they are, and these the scales of keys and values
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t meta_full[kMeta];
@@ -122,6 +124,77 @@ __device__ __forceinline__ void paged_copy_queries(const FaPagedTilesParams& p, 
   }
 }
 
+constexpr float kPagedBits = 8.f, kPagedGrowth = 7.f;  // P' is at most 2^15
+// A value scale relative to `base`, both by their bits: the difference of the exponents in place.  0 where the scale is: values are 0 then.
+__device__ __forceinline__ int paged_relative(float scale, int base) {
+  return scale != 0.f ? min(max(__float_as_int(scale) - base, -(126 << 23)), 126 << 23) : 0;
+}
+__device__ __forceinline__ float paged_log(int to) { return static_cast<float>(to >> 23); }
+__device__ __forceinline__ float paged_inverse(int to) { return __int_as_float((127 << 23) - to); }
+
+// A tile whose scales are far apart: scores with the scales of their groups, and as a function that is called, since its code in the softmax
+// loop took prompts D64 from 34.0 to 35.1 us, ragged from 105.8 to 113.0, without a single such tile.
+// Scores of 32 keys, of which half h has group 2 q + h.
+__device__ __forceinline__ void paged_group_scores(uint32_t tS, const float2* group, float factor, int lim, int q, uint32_t (&x)[32], float2 (&scale)[2],
+                                                   float (&f)[2]) {
+  tmem_ld32(tS + q * 32, x);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    scale[h] = group[2 * q + h];
+    f[h] = factor * scale[h].x;
+    f[h] = f[h] == 0.f ? 1.17549435e-38f : f[h];
+  }
+  tmem_wait_ld();
+#pragma unroll
+  for (int c = 0; c < 32; ++c) x[c] = q * 32 + c <= lim && scale[c >> 4].x != 0.f ? x[c] : 0xff800000u;
+}
+// The row's new maximum and sum, and what it falls by; P' goes to its place, which is that of scores that are read already: 16 columns for 32.
+__device__ __noinline__ float3 paged_group_softmax(uint32_t tS, const float2* group, float factor, int lim, int base, bool live, float m, float l) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int q = 0; q < kTileN / 32; ++q) {
+    uint32_t x[32];
+    float2 scale[2];
+    float f[2];
+    paged_group_scores(tS, group, factor, lim, q, x, scale, f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = __uint_as_float(x[16 * h]);
+#pragma unroll
+      for (int c = 1; c < 16; ++c) mx = fmaxf(mx, __uint_as_float(x[16 * h + c]));
+      top = fmaxf(top, fmaf(mx, f[h], paged_log(paged_relative(scale[h].y, base))));
+    }
+  }
+  const bool adopt = live && top > m + kPagedGrowth;
+  const float alpha = adopt ? fast_exp2(m - top) : 1.f;
+  m = adopt ? top : m;
+  l *= alpha;
+  const float off = kPagedBits - (m == -INFINITY ? 0.f : m);
+#pragma unroll 1
+  for (int q = 0; q < kTileN / 32; ++q) {
+    uint32_t x[32], pk[16];
+    float2 scale[2];
+    float f[2];
+    paged_group_scores(tS, group, factor, lim, q, x, scale, f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int to = paged_relative(scale[h].y, base);
+      const float off_h = off + paged_log(to);
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 16; c += 2) {
+        const float a = fast_exp2(fmaf(__uint_as_float(x[16 * h + c]), f[h], off_h));
+        const float b = fast_exp2(fmaf(__uint_as_float(x[16 * h + c + 1]), f[h], off_h));
+        sum += a + b;
+        pk[8 * h + c / 2] = scale[h].y != 0.f ? Pack2<__half>::pack(a, b) : 0u;
+      }
+      l = fmaf(sum, paged_inverse(to), l);
+    }
+    tmem_st16(tS + q * 16, pk);
+  }
+  return make_float3(m, l, alpha);
+}
+
 template <typename T, int D>
 __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, FaPagedTilesSmem<D>& s, const AbortCtx& ctx, uint32_t tmem,
                                                    const PagedItem& it, int i) {
@@ -177,7 +250,9 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     if (lane == 0) mbar_arrive(&s.q_full[i]);
   }
 
-  float m = -INFINITY, l = 0.f, v_unit = 0.f;
+  // relative to `base`, the first tile's largest value scale; l in 2^(m - kPagedBits), O in that times base
+  float m = -INFINITY, l = 0.f;
+  int base = 0;  // bits; 0: no tile yet
   for (int j = it.j0; j < n; ++j) {
     const int at = j - it.j0;
     if (!mbar_wait_warp(&s.s_full[i], at & 1, ctx, kRolePagedSoftmax)) return;
@@ -190,68 +265,69 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     const uint32_t gone = __float_as_uint(meta.z);
     tmem_wait_ld();
 
-    const int col0 = j * kTileN;
-    if (col0 + kTileN > least || gone != 0u) {
-      const int lim = limit - 1 - col0;
+    if (base == 0) base = __float_as_int(meta.y);
+    const int col0 = j * kTileN, lim = limit - 1 - col0;
+    float alpha;
+    if (meta.w != 0.f) {
+      const float3 r = paged_group_softmax(tS, s.group[at % Smem::kMeta], factor, lim, base, live, m, l);
+      m = r.x;
+      l = r.y;
+      alpha = r.z;
+    } else {
+      if (col0 + kTileN > least || gone != 0u) {
 #pragma unroll
-      for (int c = 0; c < kTileN; ++c) v[c] = (c <= lim && !((gone >> (c >> 4)) & 1u)) ? v[c] : 0xff800000u;  // -inf
-    }
-    float mx[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(v[c]);
-#pragma unroll
-    for (int c = 4; c < kTileN; c += 8) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (c + 4 < kTileN) mx[e] = max3(mx[e], __uint_as_float(v[c + e]), __uint_as_float(v[c + 4 + e]));
-        else mx[e] = fmaxf(mx[e], __uint_as_float(v[c + e]));
+        for (int c = 0; c < kTileN; ++c) v[c] = (c <= lim && !((gone >> (c >> 4)) & 1u)) ? v[c] : 0xff800000u;  // -inf
       }
-    }
-    float f = factor * meta.x;
-    f = f == 0.f ? 1.17549435e-38f : f;  // -inf has to stay it
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
-    const bool adopt = live && top > m + 7.f;  // padding rows never ask for a rescale
-    float alpha = adopt ? fast_exp2(m - top) : 1.f;
-    m = adopt ? top : m;
-    l *= alpha;
-    // P' = 2^(x f - m + e) with 2^e = 256 (the tile's value scale / the unit)
-    int e = 8;
-    if (meta.y > v_unit) {
-      alpha *= v_unit / meta.y;  // 0 at first
-      v_unit = meta.y;
-    } else if (meta.y > 0.f) {
-      e = max(8 + (__float_as_int(meta.y) >> 23) - (__float_as_int(v_unit) >> 23), -64);
-    }
-    const float off = static_cast<float>(e) - (m == -INFINITY ? 0.f : m);
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(v[c]);
+#pragma unroll
+      for (int c = 4; c < kTileN; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (c + 4 < kTileN) mx[e] = max3(mx[e], __uint_as_float(v[c + e]), __uint_as_float(v[c + 4 + e]));
+          else mx[e] = fmaxf(mx[e], __uint_as_float(v[c + e]));
+        }
+      }
+      float f = factor * meta.x;
+      f = f == 0.f ? 1.17549435e-38f : f;  // -inf has to stay it
+      const int to = paged_relative(meta.y, base);
+      const float v_log = paged_log(to);
+      const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, v_log);
+      const bool adopt = live && top > m + kPagedGrowth;  // padding rows never ask for a rescale
+      alpha = adopt ? fast_exp2(m - top) : 1.f;
+      m = adopt ? top : m;
+      const float off = v_log + kPagedBits - (m == -INFINITY ? 0.f : m);
 
-    const uint64_t f2 = pack_f32x2(f, f), off2 = pack_f32x2(off, off);
-    uint64_t sa = pack_f32x2(0.f, 0.f), sb = sa;
+      const uint64_t f2 = pack_f32x2(f, f), off2 = pack_f32x2(off, off);
+      uint64_t sa = pack_f32x2(0.f, 0.f), sb = sa;
 #pragma unroll
-    for (int q = 0; q < kTileN / 32; ++q) {
-      uint32_t pk[16];
+      for (int q = 0; q < kTileN / 32; ++q) {
+        uint32_t pk[16];
 #pragma unroll
-      for (int k = 0; k < 32; k += 4) {
-        const int c = q * 32 + k;
-        const uint64_t x0 = fma_f32x2(pack_f32x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), f2, off2);
-        const uint64_t x1 = fma_f32x2(pack_f32x2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), f2, off2);
-        float a0, a1, b0, b1;
-        unpack_f32x2(x0, a0, a1);
-        unpack_f32x2(x1, b0, b1);
-        a0 = fast_exp2(a0);
-        a1 = fast_exp2(a1);
-        b0 = fast_exp2(b0);
-        b1 = fast_exp2(b1);
-        sa = add_f32x2(sa, pack_f32x2(a0, a1));
-        sb = add_f32x2(sb, pack_f32x2(b0, b1));
-        pk[k / 2] = Pack2<__half>::pack(a0, a1);
-        pk[k / 2 + 1] = Pack2<__half>::pack(b0, b1);
+        for (int k = 0; k < 32; k += 4) {
+          const int c = q * 32 + k;
+          const uint64_t x0 = fma_f32x2(pack_f32x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), f2, off2);
+          const uint64_t x1 = fma_f32x2(pack_f32x2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), f2, off2);
+          float a0, a1, b0, b1;
+          unpack_f32x2(x0, a0, a1);
+          unpack_f32x2(x1, b0, b1);
+          a0 = fast_exp2(a0);
+          a1 = fast_exp2(a1);
+          b0 = fast_exp2(b0);
+          b1 = fast_exp2(b1);
+          sa = add_f32x2(sa, pack_f32x2(a0, a1));
+          sb = add_f32x2(sb, pack_f32x2(b0, b1));
+          pk[k / 2] = Pack2<__half>::pack(a0, a1);
+          pk[k / 2 + 1] = Pack2<__half>::pack(b0, b1);
+        }
+        tmem_st16(tS + q * 16, pk);
       }
-      tmem_st16(tS + q * 16, pk);
+      float sum0, sum1, sum2, sum3;
+      unpack_f32x2(sa, sum0, sum1);
+      unpack_f32x2(sb, sum2, sum3);
+      l = fmaf((sum0 + sum1) + (sum2 + sum3), paged_inverse(to), l * alpha);
     }
-    float sum0, sum1, sum2, sum3;
-    unpack_f32x2(sa, sum0, sum1);
-    unpack_f32x2(sb, sum2, sum3);
-    l = fmaf((sum0 + sum1) + (sum2 + sum3), __int_as_float((127 - e) << 23), l);
     // S(j) was committed behind P V(j - 1), so that product is complete, and P V(j) is only issued after this warp's arrival
     if (at > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
@@ -272,8 +348,8 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
 
   if (!mbar_wait_warp(&s.o_full[i], 0, ctx, kRolePagedSoftmax)) return;
   tc_fence_after();
-  const float inv = l != 0.f ? v_unit * (1.f / 256.f) / l : 0.f;  // a row without keys is 0, one with a NaN is NaN
-  const float lse2 = l != 0.f ? (m == -INFINITY ? 0.f : m) + fast_log2(l) : -INFINITY;
+  const float inv = l != 0.f ? __int_as_float(base) / l : 0.f;  // a row without keys is 0, one with a NaN is NaN
+  const float lse2 = l != 0.f ? (m == -INFINITY ? 0.f : m) + (fast_log2(l) - kPagedBits) : -INFINITY;
   float* part = p.part_o + (part_row - (r & 3)) * D;
 #pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
@@ -488,15 +564,22 @@ __device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p,
     const float k_inv = k_ref > 0.f ? 1.f / k_ref : 0.f, v_inv = v_ref > 0.f ? 1.f / v_ref : 0.f;
     const bool inside = j * kTileN + 16 * l8 < len;
     const uint32_t gone = __ballot_sync(0xffffffffu, inside && ks == 0.f) & 0xffu;
-    const bool k_alike = __all_sync(0xffffffffu, ks == 0.f || ks == k_ref), v_alike = __all_sync(0xffffffffu, vs == v_ref || page < 0);
+    // 2^8 apart: fp16 holds the products, and takes P' no further down than that where a row does not see the largest
+    const bool apart = __any_sync(0xffffffffu, (ks != 0.f && ks * 256.f < k_ref) || (vs != 0.f && vs * 256.f < v_ref));
+    const bool k_alike = apart || __all_sync(0xffffffffu, ks == 0.f || ks == k_ref);
+    const bool v_alike = apart || __all_sync(0xffffffffu, (vs == v_ref && vs != 0.f) || page < 0);
     const __half2 kr0 = __float2half2_rn(__shfl_sync(0xffffffffu, ks, 2 * pw) * k_inv), kr1 = __float2half2_rn(__shfl_sync(0xffffffffu, ks, 2 * pw + 1) * k_inv);
     const __half2 vr0 = __float2half2_rn(__shfl_sync(0xffffffffu, vs, 2 * pw) * v_inv), vr1 = __float2half2_rn(__shfl_sync(0xffffffffu, vs, 2 * pw + 1) * v_inv);
     if (pw == 0 && __any_sync(0xffffffffu, inside && page < 0) && lane == 0) kv_report(kv, HB_CACHE_BAD_PAGE);
 
     if (!mbar_wait_warp(&s.kv_empty[slot], phase, ctx, kRolePagedProducer)) return;
-    if (pw == 0 && lane == 0) {
-      s.meta[at] = make_float4(k_ref, v_ref, __uint_as_float(gone), 0.f);
-      mbar_arrive(&s.meta_full[at]);
+    if (pw == 0) {
+      if (apart && lane < 8) s.group[at][lane] = make_float2(ks, vs);
+      __syncwarp();
+      if (lane == 0) {
+        s.meta[at] = make_float4(k_ref, v_ref, __uint_as_float(gone), apart ? 1.f : 0.f);
+        mbar_arrive(&s.meta_full[at]);
+      }
     }
     store(slot, wk, k_alike, kr0, kr1);
     advance();

@@ -9,6 +9,8 @@ from test_paged_gpu import DT, _cache, _clean, _gen, _ints
 pytestmark = pytest.mark.gpu
 
 FEW = dict(B=5, Hkv=2, group=2)    # the rows kernel, whatever the number of tokens up to 64
+WIDE = dict(B=10, Hkv=16, group=1)  # the tiles kernel, one block an item
+LONG = dict(B=4, Hkv=8, group=4)    # the tiles kernel, keys of an item over several blocks (of long tables)
 
 
 def _reference(q, pages, table, lens, new, causal, floor):
@@ -42,8 +44,13 @@ def _reference(q, pages, table, lens, new, causal, floor):
             p = torch.exp(s - top)
             total = torch.where(some, p.sum(-1, keepdim=True), 1.0)
             o = p @ vd / total
-            # a score: D products and sums in fp32, and x f - m in fp32 (base 2)
-            err = torch.where(seen, (x.abs() @ kd.abs().T) * (D ** -0.5 * D * 2.0 ** -23) + (s.abs() + top.abs()) * 2.0 ** -22, 0.0)
+            # a score: D products and sums in fp32.  The exponent of a weight, x f + (8 - m + w) in base 2, where w is log2 of the value scale relative to
+            # another one and m a score plus such a logarithm: three roundings of fp32, each off by 2^-24 of a number of at most
+            # 1.45 (|s| + |top|) + span + 8, which moves the weight by ln 2 of that.  3 ln 2 2^-24 (1.45 (|s| + |top|) + span + 8) is less
+            # than (|s| + |top| + span) 2^-22 and the 2^-19 below
+            present = vs[h][there & (vs[h] > 0)].log2()
+            span = (present.max() - present.min()).item() if present.numel() else 0.0
+            err = torch.where(seen, (x.abs() @ kd.abs().T) * (D ** -0.5 * D * 2.0 ** -23) + (s.abs() + top.abs() + span) * 2.0 ** -22, 0.0)
             at, heads = slice(row, row + n), slice(h * group, (h + 1) * group)
             out[at, heads] = o
             moved = ((p * err) @ vd.abs() + (p * err).sum(-1, keepdim=True) * o.abs()) / total
@@ -110,6 +117,10 @@ CALLS = [  # form, new, length, page size, D, dtype, layout
     (FEW, 3, 200, 16, 64, "fp16", "bshd"),
     (FEW, 1, 1000, 32, 128, "fp16", "bhsd"),
     (FEW, 60, 130, 16, 64, "bf16", "bhsd"),
+    (WIDE, 128, 128, 16, 128, "bf16", "bhsd"),
+    (WIDE, 100, 300, 32, 64, "fp16", "bshd"),
+    (LONG, 70, 1500, 64, 128, "bf16", "bhsd"),
+    (LONG, 64, 1100, 16, 64, "fp16", "bhsd"),
 ]
 
 
@@ -131,7 +142,7 @@ def test_scales_far_apart(built_lib, form, new, length, size, D, dtype, layout, 
     _check(out, lse, _reference(q, pages, table, lens, [new] * B, True, 24))
 
 
-@pytest.mark.parametrize("form,new,length,size,D", ((FEW, 4, 100, 16, 128), (FEW, 2, 300, 32, 64)))
+@pytest.mark.parametrize("form,new,length,size,D", ((FEW, 4, 100, 16, 128), (FEW, 2, 300, 32, 64), (WIDE, 100, 300, 16, 128), (LONG, 70, 1100, 32, 64)))
 def test_scales_far_apart_among_pages_that_are_not_there(built_lib, form, new, length, size, D):
     """The same with pages of nobody's, value scales of 0, and sequences without keys; then with a NaN key and a NaN query."""
     from heddle_b200 import ops
@@ -145,6 +156,8 @@ def test_scales_far_apart_among_pages_that_are_not_there(built_lib, form, new, l
     for block in (1, 2, 5):
         table[0, block] = -1
         pages.v_scale[table[2, block].long()] = 0
+    for block in range(128 // size, min(256 // size, table.shape[1] - 1)):  # all of a tile of 128 keys
+        pages.v_scale[table[3, block].long()] = 0
     out, lse = ops.fa_paged(q, pages, table, _ints(lens), causal=False, return_lse=True)
     assert ops.cache_status() == 3 and ops.status_word() == 0  # a page outside of the cache, a sequence shorter than its rows
     live = torch.ones(B * new, dtype=torch.bool, device="cuda")
