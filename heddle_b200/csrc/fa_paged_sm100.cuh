@@ -412,9 +412,10 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       int up = 0;
       if (top > 0.f && top <= 3.402823466e38f) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
-      const float mul = __int_as_float((up + 127) << 23);
-      const unsigned votes = __ballot_sync(0xffffffffu, finite);  // a row that holds an infinity or NaN is NaN
-      const float f = ((votes >> (lane & ~3)) & 15u) == 15u ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
+      // a row that holds an infinity or NaN is NaN: its scores are, those of keys that it sees
+      const unsigned votes = __ballot_sync(0xffffffffu, finite);
+      const float mul = ((votes >> (lane & ~3)) & 15u) == 15u ? __int_as_float((up + 127) << 23) : __int_as_float(0x7fc00000);
+      const float f = p.scale_log2 * __int_as_float((127 - up) << 23);
 #pragma unroll
       for (int e = 0; e < 2; ++e) factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
 #pragma unroll

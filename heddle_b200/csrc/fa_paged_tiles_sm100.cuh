@@ -231,8 +231,9 @@ __device__ __forceinline__ void paged_softmax_role(const FaPagedTilesParams& p, 
     const bool finite = top <= 3.402823466e38f;
     int up = 0;
     if (top > 0.f && finite) up = min(14 - ((__float_as_int(top) >> 23) - 127), 120);
-    const float mul = __int_as_float((up + 127) << 23);
-    factor = finite ? p.scale_log2 * __int_as_float((127 - up) << 23) : __int_as_float(0x7fc00000);
+    // a row that holds an infinity or NaN is NaN: its scores are, those of keys that it sees
+    const float mul = finite ? __int_as_float((up + 127) << 23) : __int_as_float(0x7fc00000);
+    factor = p.scale_log2 * __int_as_float((127 - up) << 23);
 #pragma unroll
     for (int e = 0; e < D / 8; ++e) {
       const uint4 w = *rows.at(r, e);

@@ -200,3 +200,23 @@ def test_many_small_weights_beside_a_large_one(built_lib, D, dtype):
     ref = _reference(q, pages, table, [n], [1], True, 33)
     for b in range(B):
         _check(out[b:b + 1], lse[b:b + 1], ref)
+
+
+@pytest.mark.parametrize("form,new", ((FEW, 1), (FEW, 40), (WIDE, 128), (LONG, 70)))
+def test_queries_that_are_not_finite_and_see_nothing(built_lib, form, new):
+    """A row without a visible key is 0 whatever its query holds: a sequence without tokens, rows in front of the first one."""
+    from heddle_b200 import ops
+    g = _gen(199)
+    B, Hkv, group = form["B"], form["Hkv"], form["group"]
+    lens = [1000 - 11 * b for b in range(B)]
+    lens[0], lens[2] = 0, new // 2
+    pages, table = _cache(B, lens, 32, Hkv, 64, "bhsd", g)
+    q = torch.randn(B * new, Hkv * group, 64, device="cuda", generator=g).bfloat16()
+    blind = torch.zeros(B * new, dtype=torch.bool, device="cuda")
+    blind[:new] = blind[2 * new:3 * new - new // 2] = True
+    want, want_lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    q[blind, :, 3], q[blind, 0, 5] = math.nan, math.inf
+    out, lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    assert ops.cache_status() == 2 and ops.status_word() == 0
+    assert (out[blind] == 0).all() and (lse[blind] == -math.inf).all()
+    assert torch.equal(out[~blind], want[~blind]) and torch.equal(lse[~blind], want_lse[~blind])
