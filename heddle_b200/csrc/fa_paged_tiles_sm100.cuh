@@ -132,8 +132,9 @@ __device__ __forceinline__ int paged_relative(float scale, int base) {
 __device__ __forceinline__ float paged_log(int to) { return static_cast<float>(to >> 23); }
 __device__ __forceinline__ float paged_inverse(int to) { return __int_as_float((127 << 23) - to); }
 
-// A tile whose scales are far apart: scores with the scales of their groups, and as a function that is called, since its code in the softmax
-// loop took prompts D64 from 34.0 to 35.1 us, ragged from 105.8 to 113.0, without a single such tile.
+// A tile whose scales are far apart: scores with the scales of their groups.  In short loops that read the scores again, 32 at a time, and in one
+// piece beside the usual path: with a branch in front of the maximum and one in front of the weights, that path took ragged batches
+// from 106 to 113 us without a single such tile.
 // Scores of 32 keys, of which half h has group 2 q + h.
 __device__ __forceinline__ void paged_group_scores(uint32_t tS, const float2* group, float factor, int lim, int q, uint32_t (&x)[32], float2 (&scale)[2],
                                                    float (&f)[2]) {
@@ -149,7 +150,7 @@ __device__ __forceinline__ void paged_group_scores(uint32_t tS, const float2* gr
   for (int c = 0; c < 32; ++c) x[c] = q * 32 + c <= lim && scale[c >> 4].x != 0.f ? x[c] : 0xff800000u;
 }
 // The row's new maximum and sum, and what it falls by; P' goes to its place, which is that of scores that are read already: 16 columns for 32.
-__device__ __noinline__ float3 paged_group_softmax(uint32_t tS, const float2* group, float factor, int lim, int base, bool live, float m, float l) {
+__device__ __forceinline__ float3 paged_group_softmax(uint32_t tS, const float2* group, float factor, int lim, int base, bool live, float m, float l) {
   float top = -INFINITY;
 #pragma unroll 1
   for (int q = 0; q < kTileN / 32; ++q) {
@@ -566,9 +567,14 @@ __device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p,
     const bool inside = j * kTileN + 16 * l8 < len;
     const uint32_t gone = __ballot_sync(0xffffffffu, inside && ks == 0.f) & 0xffu;
     // 2^8 apart: fp16 holds the products, and takes P' no further down than that where a row does not see the largest
-    const bool apart = __any_sync(0xffffffffu, (ks != 0.f && ks * 256.f < k_ref) || (vs != 0.f && vs * 256.f < v_ref));
-    const bool k_alike = apart || __all_sync(0xffffffffu, ks == 0.f || ks == k_ref);
-    const bool v_alike = apart || __all_sync(0xffffffffu, (vs == v_ref && vs != 0.f) || page < 0);
+    bool k_alike = __all_sync(0xffffffffu, ks == 0.f || ks == k_ref);
+    bool v_alike = __all_sync(0xffffffffu, (vs == v_ref && vs != 0.f) || page < 0);
+    bool apart = false;
+    if (!(k_alike && v_alike)) {  // asked only here: D128 chunks with pages of 16 133.6 us, with the question in front of every tile 136.9
+      apart = __any_sync(0xffffffffu, (ks != 0.f && ks * 256.f < k_ref) || (vs != 0.f && vs * 256.f < v_ref));
+      k_alike = k_alike || apart;
+      v_alike = v_alike || apart;
+    }
     const __half2 kr0 = __float2half2_rn(__shfl_sync(0xffffffffu, ks, 2 * pw) * k_inv), kr1 = __float2half2_rn(__shfl_sync(0xffffffffu, ks, 2 * pw + 1) * k_inv);
     const __half2 vr0 = __float2half2_rn(__shfl_sync(0xffffffffu, vs, 2 * pw) * v_inv), vr1 = __float2half2_rn(__shfl_sync(0xffffffffu, vs, 2 * pw + 1) * v_inv);
     if (pw == 0 && __any_sync(0xffffffffu, inside && page < 0) && lane == 0) kv_report(kv, HB_CACHE_BAD_PAGE);
