@@ -179,10 +179,12 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
 
   // ---- this block's run of the list: the sequences' parts are added up in rounds of a block's threads
   long long total = 0, own = 0, upto = 0;  // own: of the last round
+  bool descends = false;                   // see kv_descends
   for (int b0 = 0; b0 < kv.B; b0 += kPagedThreads) {
     const int b = b0 + threadIdx.x;
     int tiles, row_tiles;
     own = upto = b < kv.B ? paged_list(p, kv_seq(kv, b), kRows, kTile, tiles, row_tiles) : 0;
+    const bool down = kv.starts != nullptr && b < kv.B && kv_start(kv, b) > kv_start(kv, b + 1);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, upto, o);
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     }
     if (b0 > 0) __syncthreads();
     if (lane == 31) sm.sums[warp] = upto;
-    __syncthreads();
+    if (__syncthreads_or(down)) descends = true;
     upto += total;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) {
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     }
   }
   const int runs = paged_runs(total, gridDim.x);
-  if (total == 0 || run >= runs) return;
+  if (total == 0 || run >= runs || descends) return;
   const long long begin = paged_begin(total, runs, run), end = paged_begin(total, runs, run + 1);
   if (kv.B <= kPagedThreads) {
     if (upto > begin && upto - own <= begin) {

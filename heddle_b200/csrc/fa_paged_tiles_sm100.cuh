@@ -68,7 +68,7 @@ struct FaPagedTilesSmem {
   uint64_t drain;
   long long sums[kPagedTilesThreads / 32];
   long long found_at;
-  int found;
+  int found, descends;
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
@@ -610,6 +610,7 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
     s.found = -1;
+    s.descends = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 4);
       mbar_init(&s.s_full[i], 1);
@@ -642,9 +643,10 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
       s.found = 0;
       s.found_at = 0;
     }
-    for (int b0 = kv.starts == nullptr ? kv.B : 0; b0 < kv.B && before <= index; b0 += kPagedTilesThreads) {
+    for (int b0 = kv.starts == nullptr ? kv.B : 0; b0 < kv.B; b0 += kPagedTilesThreads) {
       const int b = b0 + threadIdx.x;
       const long long own = b < kv.B ? static_cast<long long>(paged_blocks_of(p, kv_seq(kv, b))) * kv.Hkv : 0;
+      if (b < kv.B && kv_start(kv, b) > kv_start(kv, b + 1)) s.descends = 1;  // see kv_descends
       long long upto = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(kPagedTilesThreads, 1) fa_paged_tiles_kernel(c
       }
     }
     __syncthreads();
-    if (s.found < 0) {  // the grid is cut for the most items that so many rows can be
+    if (s.found < 0 || s.descends != 0) {  // the grid is cut for the most items that so many rows can be
       if (p.splits > 1 && split == 0 && threadIdx.x == 0) p.parts[index].count = 0;
       if (p.chained) grid_wait();
       return;

@@ -165,6 +165,14 @@ __device__ __forceinline__ void append_queries(const KvAppendParams& p) {
 template <typename T, int D, int GS>
 __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
   grid_wait();
+  if (p.c.starts != nullptr && __syncthreads_or(kv_descends(p.c))) {
+    if (blockIdx.x == 0)
+      for (int b = threadIdx.x; b < p.c.B; b += kAppendThreads) {
+        const uint32_t f = kv_seq_faults(p.c, b);
+        if (f != 0) kv_report(p.c, f);
+      }
+    return;
+  }
   if (static_cast<int>(blockIdx.x) >= p.cache_blocks) {
     append_queries<T, D>(p);
     return;

@@ -99,6 +99,14 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& c, int b) {
   s.len = min(max(c.lens[b], 0), c.max_pages << c.page_shift);
   return s;
 }
+// Whether starts descend somewhere, of what this thread of a block looks at; the threads together look at all of them.  A call whose starts do
+// has rows that belong to two sequences: it reports that and writes nothing.
+__device__ __forceinline__ bool kv_descends(const KvView& c) {
+  bool down = false;
+  if (c.starts != nullptr)
+    for (int b = threadIdx.x; b < c.B; b += blockDim.x) down = down || kv_start(c, b) > kv_start(c, b + 1);
+  return down;
+}
 // What of sequence b kv_seq had to mend.
 __device__ __forceinline__ uint32_t kv_seq_faults(const KvView& c, int b) {
   const KvSeq s = kv_seq(c, b);

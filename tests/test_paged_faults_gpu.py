@@ -1,0 +1,60 @@
+"""What the paged cache's kernels do with tables, lengths and starts that are wrong: what they write, what they leave, what they report."""
+import pytest
+import torch
+
+from oracle import paged_oracle as P
+from test_paged_gpu import _cache, _gen, _ints, _rope
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(a, b):
+    return all(torch.equal(torch.nan_to_num(x, nan=1e9), torch.nan_to_num(y, nan=1e9)) for x, y in zip(a.codes + a.scales, b.codes + b.scales))
+
+
+DESCENDING = [  # starts, rows, tokens of each sequence, page size, Hkv
+    ([0, 100, 0, 100], 100, 200, 16, 2),
+    ([0, 3, 1, 4], 4, 50, 16, 1),
+    ([0, 300, 299, 600], 600, 700, 64, 4),
+    ([5, 4] + [6] * 299, 6, 40, 32, 2),   # more sequences than a block of the rows kernel has threads, the first one wrong
+    ([0] * 299 + [70, 69], 70, 90, 32, 2),  # the last one
+]
+
+
+@pytest.mark.parametrize("starts,T,length,size,Hkv", DESCENDING)
+def test_starts_that_descend(built_lib, starts, T, length, size, Hkv):
+    """Nothing is written, neither to the cache nor to the outputs, and it is reported, by append too."""
+    from heddle_b200 import ops
+    g = _gen(211)
+    B, D = len(starts) - 1, 64
+    lens = [length] * B
+    pages, table = _cache(B, lens, size, Hkv, D, "bhsd", g)
+    before = P.Cache(pages)
+    k, v, q = (torch.randn(T, H, D, device="cuda", generator=g).bfloat16() for H in (Hkv, Hkv, 2 * Hkv))
+    ops.kv_append(k, v, pages, table, _ints(lens), starts=_ints(starts), rope=_rope(length, D), q=q)
+    assert ops.cache_status() == 4
+    assert _same(before, P.Cache(pages))
+    for hint in (None, T, 1):
+        out = torch.full_like(q, 7.0)
+        ops.fa_paged(q, pages, table, _ints(lens), starts=_ints(starts), max_tokens=hint, out=out)
+        assert ops.cache_status() == 4 and ops.status_word() == 0
+        assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("n,Hkv", ((2, 1), (150, 8)))
+def test_starts_that_leave_the_rows(built_lib, n, Hkv):
+    """They are taken as the nearest that do not: the first and last row."""
+    from heddle_b200 import ops
+    g = _gen(223)
+    D, size, lens = 64, 16, [n + 40, n + 30, n + 33]
+    pages, table = _cache(3, lens, size, Hkv, D, "bhsd", g)
+    copy = pages._replace(**{name: getattr(pages, name).clone() for name in ("k", "v", "k_scale", "v_scale")})
+    k, v, q = (torch.randn(3 * n, H, D, device="cuda", generator=g).bfloat16() for H in (Hkv, Hkv, 2 * Hkv))
+    results = []
+    for where, starts, status in ((pages, [0, n, 2 * n, 3 * n], 0), (copy, [-5, n, 2 * n, 1 << 30], 4)):
+        turned = ops.kv_append(k, v, where, table, _ints(lens), starts=_ints(starts), q=q)
+        assert ops.cache_status() == status
+        results.append((turned, ops.fa_paged(turned, where, table, _ints(lens), starts=_ints(starts))))
+        assert ops.cache_status() == status
+    assert _same(P.Cache(pages), P.Cache(copy))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
