@@ -137,8 +137,9 @@ __device__ __forceinline__ void append_queries(const KvAppendParams& p) {
     lo4[k] = *reinterpret_cast<const uint4*>(src);
     hi4[k] = *reinterpret_cast<const uint4*>(src + D / 2);
     dst[k] = static_cast<T*>(p.q_out) + t * p.qo_st + head * p.qo_sh + piece * 8;
-    const KvSeq s = kv_seq(p.c, append_seq_of(p, t));
-    const int at = t - s.start, x = s.pos0() + at;
+    const int b = append_seq_of(p, t);
+    const KvSeq s = kv_seq(p.c, b);
+    const int at = t - s.start, x = kv_append_position(p.c, b, s) + at;
     // not a row of no sequence, nor one behind the tables (reported with the keys)
     if (at >= 0 && at < s.n && (p.cos == nullptr || (x >= 0 && x < p.rope_len))) pos[k] = max(x, 0);
   }
@@ -200,13 +201,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __gr
     block = slot - ((kv_start(c, b) >> c.page_shift) + 2 * b);
   }
   const KvSeq s = kv_seq(c, b);
-  const int pos0 = s.pos0();
+  const int pos0 = kv_append_position(c, b, s);
   if (h == 0 && block == 0 && tid == 0) {
     uint32_t f = kv_seq_faults(c, b);
-    if (p.cos != nullptr && s.n > 0 && s.len > p.rope_len) f |= HB_CACHE_BAD_POSITION;
+    if (p.cos != nullptr && s.n > 0 && pos0 + s.n > p.rope_len) f |= HB_CACHE_BAD_POSITION;
     if (f != 0) kv_report(c, f);
   }
-  const int limit = p.cos != nullptr ? min(s.len, p.rope_len) : s.len;  // tokens behind the tables are not written
+  const int limit = p.cos != nullptr ? min(s.len, p.rope_len) : s.len;  // tokens behind the tables, of pages or of angles, are not written
   block += max(pos0, 0) >> c.page_shift;
   if (block < 0 || block >= c.max_pages) return;
   const int begin = block << c.page_shift;

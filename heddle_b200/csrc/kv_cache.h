@@ -99,6 +99,8 @@ __device__ __forceinline__ KvSeq kv_seq(const KvView& c, int b) {
   s.len = min(max(c.lens[b], 0), c.max_pages << c.page_shift);
   return s;
 }
+// The position that the sequence's first row is appended at: a length behind the page table's end moves no token in front of it.
+__device__ __forceinline__ int kv_append_position(const KvView& c, int b, const KvSeq& s) { return max(c.lens[b], 0) - s.n; }
 // Whether starts descend somewhere, of what this thread of a block looks at; the threads together look at all of them.  A call whose starts do
 // has rows that belong to two sequences: it reports that and writes nothing.
 __device__ __forceinline__ bool kv_descends(const KvView& c) {

@@ -467,8 +467,8 @@ int hb_debug_rowwise_compile(const hb_rowwise_args* args, char* source, int64_t 
  * page_table, seq_lens and starts are read on the device: a captured call takes what they hold when it is replayed.  Entries of the
  * page table behind a sequence's last page are not read.  What the device finds wrong in them it leaves out and reports
  * through hb_cache_status: a page outside of [0, num_pages) (its tokens are not written, and are not seen by any query), a
- * length beyond max_pages * page_size (taken as that), more rows than the sequence is long, a position behind the rotary tables
- * (neither written), starts that leave [0, T] (taken as the nearest that do not).  Where starts then descend, rows would belong to two
+ * length beyond max_pages * page_size (attention takes it as that, append leaves out the tokens behind it), more rows than the sequence
+ * is long, a position behind the rotary tables (neither written), starts that leave [0, T] (taken as the nearest that do not).  Where starts then descend, rows would belong to two
  * sequences: such a call writes nothing at all, and is reported.
  * page_size 16, 32, 64 or 128; D 64 or 128.
  */

@@ -58,3 +58,34 @@ def test_starts_that_leave_the_rows(built_lib, n, Hkv):
         assert ops.cache_status() == status
     assert _same(P.Cache(pages), P.Cache(copy))
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
+OVERLONG = [  # new tokens, tokens that the lengths give the sequences, columns of the table, page size
+    ([1, 1, 1], [49, 48, 200], 3, 16),
+    ([5, 5], [66, 64], 2, 32),
+    ([100, 30, 1], [150, 130, (1 << 31) - 1], 1, 128),
+]
+
+
+@pytest.mark.parametrize("rotate", (True, False))
+@pytest.mark.parametrize("new,lens,columns,size", OVERLONG)
+def test_append_behind_the_page_table(built_lib, new, lens, columns, size, rotate):
+    """Tokens behind the last page of the table are left out; those in front of them keep their places and angles."""
+    from heddle_b200 import ops
+    g = _gen(227)
+    B, Hkv, D = len(new), 2, 64
+    pages, table = _cache(B, [columns * size] * B, size, Hkv, D, "bhsd", g)
+    table = table[:, :columns].contiguous()
+    k, v, q = (torch.randn(sum(new), H, D, device="cuda", generator=g).bfloat16() for H in (Hkv, Hkv, 4))
+    starts, rope = torch.tensor([0] + new).cumsum(0).int().cuda(), _rope(250, D) if rotate else None
+    want = P.Cache(pages)
+    want.append(k, v, table.cpu(), lens, starts.tolist(), rope)
+    turned = ops.kv_append(k, v, pages, table, _ints(lens), starts=starts, rope=rope, q=q)
+    assert ops.cache_status() == (10 if rotate and max(lens) > 250 else 2)
+    assert _same(want, P.Cache(pages))
+    # the queries: as with a table that is long enough
+    wide = torch.cat([table, torch.full((B, 8), -1, dtype=torch.int32, device="cuda")], 1).contiguous()
+    again = ops.kv_append(k, v, pages, wide, _ints([min(n, 250) for n in lens]), starts=starts, rope=rope, q=q)
+    ops.cache_status()
+    for b in (b for b, n in enumerate(lens) if n <= 250):
+        assert torch.equal(turned[starts[b]:starts[b + 1]], again[starts[b]:starts[b + 1]])
