@@ -72,8 +72,8 @@ int get_device_state(DeviceState** out) {
                        "device %d has compute capability %d.%d; this library is built for sm_100a only", dev, major,
                        minor);
     }
-    HB_CUDA_CHECK(cudaMalloc(&st.status_word, 2 * sizeof(uint32_t)));
-    HB_CUDA_CHECK(cudaMemset(st.status_word, 0, 2 * sizeof(uint32_t)));
+    HB_CUDA_CHECK(cudaMalloc(&st.status_word, 3 * sizeof(uint32_t)));  // and two for hb_cache_status
+    HB_CUDA_CHECK(cudaMemset(st.status_word, 0, 3 * sizeof(uint32_t)));
     st.cache_fault = st.status_word + 1;
     st.device = dev;
   }
@@ -142,6 +142,9 @@ int encode_tensor_map(CUtensorMap* out, CUtensorMapDataType dt, int rank, const 
   return HB_OK;
 }
 
+// Reads and clears in one: kernels of other threads and streams may report meanwhile, and what they do is left for the next reading.
+static __global__ void take_word(uint32_t* word, uint32_t* taken) { *taken = atomicExch(word, 0u); }
+
 }  // namespace hb
 
 extern "C" {
@@ -168,10 +171,15 @@ int hb_cache_status(uint32_t* out) {
   hb::DeviceState* st = nullptr;
   int rc = hb::get_device_state(&st);
   if (rc != HB_OK) return rc;
-  HB_CUDA_CHECK(cudaDeviceSynchronize());
-  HB_CUDA_CHECK(cudaMemcpy(out, st->cache_fault, sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  static std::mutex mutex;  // of the word that the fault is taken into
+  {
+    std::lock_guard<std::mutex> lock(mutex);
+    HB_CUDA_CHECK(cudaDeviceSynchronize());
+    hb::take_word<<<1, 1>>>(st->cache_fault, st->cache_fault + 1);
+    HB_CUDA_CHECK(cudaGetLastError());
+    HB_CUDA_CHECK(cudaMemcpy(out, st->cache_fault + 1, sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  }
   if (*out == 0) return HB_OK;
-  HB_CUDA_CHECK(cudaMemset(st->cache_fault, 0, sizeof(uint32_t)));
   return hb::set_error(HB_ERR_BAD_ARG, "hb_cache_status: 0x%x:%s%s%s%s", *out,
                        *out & HB_CACHE_BAD_PAGE ? " a page outside of the cache;" : "",
                        *out & HB_CACHE_BAD_LENGTH ? " a length that does not fit its page table row or its tokens;" : "",

@@ -89,3 +89,47 @@ def test_append_behind_the_page_table(built_lib, new, lens, columns, size, rotat
     ops.cache_status()
     for b in (b for b, n in enumerate(lens) if n <= 250):
         assert torch.equal(turned[starts[b]:starts[b + 1]], again[starts[b]:starts[b + 1]])
+
+
+def test_reports_are_not_lost_while_others_are_read(built_lib):
+    """One thread has two faults found, one after the other, again and again; another one reads all the time, and gets each."""
+    import threading
+    import time
+
+    from heddle_b200 import ops
+    pages, table = _cache(1, [16], 16, 1, 64, "bhsd", _gen(229))
+    nowhere, q = torch.full_like(table, -1), torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    fine, longer = _ints([16]), _ints([17 * table.shape[1]])
+    torch.cuda.synchronize()
+    reads, stop, failed = [], threading.Event(), []
+
+    def reader():
+        try:
+            while not stop.is_set():
+                reads.append(ops.cache_status())
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    thread = threading.Thread(target=reader)
+    thread.start()
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for n in range(1500):
+                before = len(reads)
+                ops.fa_paged(q, pages, nowhere, fine)   # a page outside of the cache
+                for _ in range(n % 7):
+                    time.sleep(0)
+                ops.fa_paged(q, pages, table, longer)   # a length behind the table
+                torch.cuda.current_stream().synchronize()
+                got, until = 0, time.monotonic() + 2
+                while got != 3 and time.monotonic() < until and not failed:
+                    got = 0
+                    for bits in reads[max(before - 1, 0):]:  # the last one may have begun before
+                        got |= bits
+                assert got == 3, (n, got)
+                while len(reads) < before + 4 and time.monotonic() < until and not failed:  # nothing of this round is left for the next one
+                    pass
+    finally:
+        stop.set()
+        thread.join()
+    assert not failed and set(reads) <= {0, 1, 2, 3}
