@@ -226,7 +226,6 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
   if (route.rows_kernel) {
     fill(p);
     p.row_limit = route.tiles_kernel ? route.row_limit : INT_MAX;
-    p.chained = route.tiles_kernel ? 1 : 0;
     p.status = st->status_word;
     for (const bool keys : {true, false}) {
       // an axis of one page, head or token may carry any stride
@@ -252,7 +251,6 @@ extern "C" int hb_fa_paged(const hb_fa_paged_args* a, void* workspace, uint64_t 
     t.row_limit = route.row_limit;
     t.by_hkv = make_fast_div(c.Hkv);
     t.by_b = make_fast_div(c.B);
-    t.chained = route.rows_kernel ? 1 : 0;
     t.status = st->status_word;
     t.splits = route.splits;
     t.parts = static_cast<PagedParts*>(workspace);

@@ -52,7 +52,6 @@ struct alignas(64) FaPagedParams {
   long long q_st, q_sh, o_st, o_sh;
   int Hq, group, causal;
   int row_limit;    // sequences with more query rows a KV head are not this kernel's
-  int chained;      // the tiles kernel of the same call follows, and runs beside this one
   FastDiv by_group;
   float scale_log2;
   uint32_t* status;
@@ -175,7 +174,6 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     prefetch_tensormap(&p.tm_v);
   }
   grid_wait();
-  if (p.chained) grid_launch_dependents();
 
   // ---- this block's run of the list: the sequences' parts are added up in rounds of a block's threads
   long long total = 0, own = 0, upto = 0;  // own: of the last round
