@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
       for (int t = 0; t < kGroups; ++t) {
         there = there && ks[t] != 0.f;
         valued = valued && vs[t] != 0.f;
-        v_top = max(v_top, __float_as_int(vs[t]));
+        v_top = max(v_top, ks[t] != 0.f ? __float_as_int(vs[t]) : 0);
       }
       if (base == 0) base = v_top;
       if ((j + 1) * kTile > least || !there) {

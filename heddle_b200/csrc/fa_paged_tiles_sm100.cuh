@@ -556,6 +556,7 @@ __device__ __forceinline__ void paged_producer_role(const FaPagedTilesParams& p,
     const int next = page_of(j + 1);
     fetch(v_base, kv.v_sp, kv.v_ss, j, page, wv);
     // the tile's largest scales, and this warp's two halves relative to them
+    if (ks == 0.f) vs = 0.f;
     float k_ref = ks, v_ref = vs;
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {

@@ -470,6 +470,8 @@ int hb_debug_rowwise_compile(const hb_rowwise_args* args, char* source, int64_t 
  * length beyond max_pages * page_size (attention takes it as that, append leaves out the tokens behind it), more rows than the sequence
  * is long, a position behind the rotary tables (neither written), starts that leave [0, T] (taken as the nearest that do not).  Where starts then descend, rows would belong to two
  * sequences: such a call writes nothing at all, and is reported.
+ * A page whose key scale is 0 in a head holds nothing there yet, as every page before its first append: it is not seen either, and that
+ * is not reported.  A value scale of 0 makes the page's values 0.
  * page_size 16, 32, 64 or 128; D 64 or 128.
  */
 typedef struct hb_kv_cache {
@@ -493,7 +495,7 @@ typedef struct hb_kv_cache {
  * largest magnitude to at most 448; in a page that holds earlier tokens of the sequence the scale grows where the new ones
  * need it, and the earlier codes are then rounded again to the new scale.  A token whose key or value holds an infinity or
  * a NaN (or whose key does once rotated) becomes a NaN key and a zero value in that head: a query that sees it is NaN, no other.
- * A page takes tokens of one sequence in a call; no other work may use its pages meanwhile.
+ * A page takes tokens of one sequence, at one place of its table row, in a call; no other work may use its pages meanwhile.
  *   k, v   [T, Hkv, D]; q (may be NULL) [T, Hq, D], rotated into q_out [T, Hq, D] (may be q itself); 16-bit, by strides
  *   rope_cos, rope_sin  fp32 [rope_len, D / 2] contiguous, indexed by position; both NULL: nothing is rotated
  * Rotation pairs i with i + D/2: x_i cos - x_{i+D/2} sin and x_{i+D/2} cos + x_i sin, products and sums rounded to fp32 each.

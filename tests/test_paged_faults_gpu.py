@@ -133,3 +133,25 @@ def test_reports_are_not_lost_while_others_are_read(built_lib):
         stop.set()
         thread.join()
     assert not failed and set(reads) <= {0, 1, 2, 3}
+
+
+@pytest.mark.parametrize("B,new,length,size,Hkv,group,D", ((3, 1, 300, 16, 2, 4, 128), (3, 7, 200, 64, 2, 4, 64), (10, 70, 300, 16, 16, 1, 128), (4, 64, 1500, 64, 8, 4, 64)))
+@pytest.mark.parametrize("value_scale", (float("nan"), float("inf"), 2.0 ** 100, 0.0))
+def test_a_page_whose_key_scale_is_zero_is_not_there(built_lib, B, new, length, size, Hkv, group, D, value_scale):
+    """A page that nothing was written to yet: not seen, whatever its value scale is, and not reported."""
+    from heddle_b200 import ops
+    g = _gen(233)
+    lens = [length - 5 * b for b in range(B)]
+    pages, table = _cache(B, lens, size, Hkv, D, "bhsd", g)
+    q = torch.randn(B * new, Hkv * group, D, device="cuda", generator=g).bfloat16()
+    gone = [(0, 0), (0, 2), (1, 1), (1, (lens[1] - 1) // size), *((2, block) for block in range(128 // size))]
+    for b, block in gone:
+        pages.k_scale[int(table[b, block])] = 0
+        pages.v_scale[int(table[b, block])] = value_scale
+    out, lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    assert ops.cache_status() == 0 and ops.status_word() == 0
+    for b, block in gone:
+        table[b, block] = -1
+    want, want_lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    assert ops.cache_status() == 1 and ops.status_word() == 0
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
