@@ -20,8 +20,8 @@
 // Work: the list of fa_paged_plan.h.  A run may start or end inside an item: such a segment leaves fp32 partial results in the
 // workspace, and fa_paged_combine_kernel merges them.
 //
-// us of GPU time, both kernels (bytes the call cannot do without): B64 Hq32 Hkv8 D128, one token, 2000 to 4100 keys 70.2 (406 MB, 5.8 TB/s); B3 Hq64 Hkv8 D128,
-// 30 to 60 thousand keys 53.0 (5.3 TB/s); B24 Hq32 Hkv8 D128, four tokens, 1500 to 3000 keys 34.7 (3.3); B40 Hq12 Hkv12 D64 25.8 (3.2); B1, 1000 keys 8.8.
+// us in a captured graph, both kernels (bytes the call cannot do without): B64 Hq32 Hkv8 D128, one token, 2000 to 4100 keys 69.7 (406 MB, 5.8 TB/s); B3 Hq64
+// Hkv8 D128, 30 to 60 thousand keys 52.8 (5.3 TB/s); B24 Hq32 Hkv8 D128, four tokens, 1500 to 3000 keys 34.4 (3.3); B40 Hq12 Hkv12 D64 26.4 (3.1); B1, 1000 keys 8.6.
 // About 10 us of each are the start (list, first pages), the meeting of the warps and the merge; the loop itself reads 5 to 6 TB/s.
 #pragma once
 

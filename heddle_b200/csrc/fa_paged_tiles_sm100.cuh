@@ -14,8 +14,8 @@
 // A row's maximum is that of score + log2 value scale, adopted when it grew by more than 2^7 (fa_paged_sm100.cuh).  O is rescaled by the row's
 // own thread, as in fa_split.
 //
-// us of GPU time: B2 Hq32 Hkv8 D128, 2048 queries behind 6144 505 (0.94 PFLOP/s; tensor pipe and MUFU 48 % each, at the power cap, as fa_fwd); B4 Hq16
-// Hkv16 D64, prompts of 1024 33.6; B16 Hq28 Hkv4 D128, 1 to 400 queries behind 750 to 1500 104.3.  The short ones pay for starts and ends of blocks.
+// us in a captured graph: B2 Hq32 Hkv8 D128, 2048 queries behind 6144 507 (0.93 PFLOP/s; tensor pipe and MUFU 48 % each); B4 Hq16
+// Hkv16 D64, prompts of 1024 33.9; B16 Hq28 Hkv4 D128, 1 to 400 queries behind 750 to 1500 105.3.  The short ones pay for starts and ends of blocks.
 #pragma once
 
 #include "fa_fwd_sm100.cuh"

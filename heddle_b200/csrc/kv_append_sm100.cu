@@ -8,7 +8,7 @@
 // that fall below e4m3's smallest step.  They grow only where a new token needs it, so that a decode step nearly always writes its
 // own 2 D bytes and leaves the page alone.
 //
-// What bounds it: HBM.  Four prompts of 2048 tokens with their queries (Hq32 Hkv8 D128 bf16, 189 MB) 37.3 us, 5.1 TB/s; one token for 64 sequences 3.5 us,
+// What bounds it: HBM.  Four prompts of 2048 tokens with their queries (Hq32 Hkv8 D128 bf16, 189 MB) 37.4 us in a captured graph, 5.0 TB/s; one token for 64 sequences 3.5 us,
 // a launch and a chain of four loads.
 #include "host_common.h"
 #include "fast_div.h"
