@@ -523,7 +523,7 @@ int hb_kv_append(const hb_kv_append_args* args);
  * Queries go into the product as fp16, each row scaled by a power of two that takes its largest element near 2^15 (what lies 2^-39 below
  * it is lost), keys and values as fp16 exactly; scores and sums are fp32.  A row's weights are rounded to fp16 in proportion to the largest
  * product of weight and value scale among the keys that it sees: a key whose own is 2^-25 of that or less may count as 0 in O.  Pages that it
- * does not see have no part in that.  Value scales may lie up to 2^126 apart.  Which SM has which keys follows from the arguments, from
+ * does not see have no part in that.  Value scales may lie up to 2^100 apart.  Which SM has which keys follows from the arguments, from
  * seq_lens and starts and from the device's SMs: results repeat for equal ones, and agree within rounding between batches.
  * A NaN code among the values of a page may reach every query whose tile of keys holds it: hb_kv_append writes none.
  *   max_tokens  the most rows of a sequence (a hint: it chooses kernels, any value gives the result); <= 0: unknown

@@ -220,3 +220,23 @@ def test_queries_that_are_not_finite_and_see_nothing(built_lib, form, new):
     assert ops.cache_status() == 2 and ops.status_word() == 0
     assert (out[blind] == 0).all() and (lse[blind] == -math.inf).all()
     assert torch.equal(out[~blind], want[~blind]) and torch.equal(lse[~blind], want_lse[~blind])
+
+
+@pytest.mark.parametrize("form,new,length,size,D,dtype,layout", CALLS)
+@pytest.mark.parametrize("where", ("first", "last", "between"))
+def test_pages_of_zeros(built_lib, form, new, length, size, D, dtype, layout, where):
+    """Values of zero, as kv_append stores them, with the smallest scale there is, beside ordinary ones with scales of 2^-6 and 1."""
+    from heddle_b200 import ops
+    g = _gen(241)
+    B, Hkv, group = form["B"], form["Hkv"], form["group"]
+    lens = [max(length - b, new) for b in range(B)]
+    pages, table = _cache(B, lens, size, Hkv, D, layout, g)
+    columns = table.shape[1]
+    blocks = {"first": range((columns + 1) // 2), "last": range(columns // 2, columns), "between": range(columns // 3, columns, 3)}[where]
+    _blocks(pages, table, 1, lambda block, _: -100 if block in blocks else -6 if block % 2 else 0)
+    for block in blocks:
+        pages.v.view(torch.uint8)[table[:, block].long()] = 0
+    q = torch.randn(B * new, Hkv * group, D, device="cuda", generator=g).to(DT[dtype])
+    out, lse = ops.fa_paged(q, pages, table, _ints(lens), return_lse=True)
+    _clean()
+    _check(out, lse, _reference(q, pages, table, lens, [new] * B, True, 24))
