@@ -34,6 +34,7 @@ namespace hb {
 constexpr int kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedMaxRows = 16;
 constexpr uint32_t kRolePagedRows = 14;
+constexpr float kPagedBits = 8.f, kPagedGrowth = 7.f;  // P' = 2^(kPagedBits + score - m): at most 2^15, since m is adopted behind kPagedGrowth
 
 struct alignas(16) PagedHead {  // of an item in parts: where its parts lie (one a run; written by the run that starts the item)
   int last;         // run of its last part, -1: this run starts no item in parts
@@ -158,7 +159,6 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
   constexpr int kSteps = D / 16;  // products along head_dim
   constexpr int kDims = D / 16;   // accumulator tiles of O^T along head_dim
   constexpr int kN = kRows / 8;   // tiles of query rows
-  constexpr float kGrowth = 7.f, kPBits = 8.f;  // P' is at most 2^15
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
     const int least = p.causal ? min(seg.s.len, seg.s.pos0() + fast_div(row0, p.by_group) + 1) : seg.s.len;
 
     float o[kN][kDims][4];
-    // value scales are relative to `base`, the first tile's largest; m: the largest score + log2 vscale / base; O is in 2^(m - kPBits) base, l in
-    // 2^(m - kPBits)
+    // value scales are relative to `base`, the first tile's largest; m: the largest score + log2 vscale / base; O is in 2^(m - kPagedBits) base, l in
+    // 2^(m - kPagedBits)
     float m[kN][2], l[kN][2];
     int base = 0;  // bits; 0: no tile yet
 #pragma unroll
@@ -527,12 +527,12 @@ __global__ void __launch_bounds__(kPagedThreads, (paged_blocks_per_sm<D, kRows>)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const bool adopt = top > m[n][e] + kGrowth;  // of -inf: any maximum
+          const bool adopt = top > m[n][e] + kPagedGrowth;  // of -inf: any maximum
           alpha[n][e] = adopt ? fast_exp2(m[n][e] - top) : 1.f;
           moved = moved || adopt;
           m[n][e] = adopt ? top : m[n][e];
-          // the 2^kPBits go in here, in front of the rounding to fp16: its numbers below 2^-14 lose bits, those below 2^-25 are 0
-          const float off = kPBits - (m[n][e] == -INFINITY ? 0.f : m[n][e]);
+          // the 2^kPagedBits go in here, in front of the rounding to fp16: its numbers below 2^-14 lose bits, those below 2^-25 are 0
+          const float off = kPagedBits - (m[n][e] == -INFINITY ? 0.f : m[n][e]);
           float sum = 0.f;
 #pragma unroll
           for (int t = 0; t < kGroups; ++t) {

@@ -123,7 +123,6 @@ __device__ __forceinline__ void paged_copy_queries(const FaPagedTilesParams& p, 
   }
 }
 
-constexpr float kPagedBits = 8.f, kPagedGrowth = 7.f;  // P' is at most 2^15
 // A value scale relative to `base`, both by their bits: the difference of the exponents in place.  0 where the scale is: values are 0 then.
 __device__ __forceinline__ int paged_relative(float scale, int base) {
   return scale != 0.f ? min(max(__float_as_int(scale) - base, -(126 << 23)), 126 << 23) : 0;

@@ -678,7 +678,8 @@ def h2o_score(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, causal: bo
 class KvPages(NamedTuple):
     """Pages of a key/value cache: e4m3 codes and a power-of-two fp32 scale for each (page, head).  ``layout`` "bhsd": ``k`` and ``v``
     are [num_pages, Hkv, page_size, D]; "bshd": [num_pages, page_size, Hkv, D]; any strides, head_dim contiguous.  The scales are
-    [num_pages, Hkv], contiguous; a key scale of 0 says that nothing was written there yet, and no query sees such a page.  Token t of sequence b is in page ``page_table[b, t // page_size]``, at place ``t % page_size``."""
+    [num_pages, Hkv], contiguous; a key scale of 0 says that nothing was written there yet, and no query sees such a page.  Token t of
+    sequence b is in page ``page_table[b, t // page_size]``, at place ``t % page_size``."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor

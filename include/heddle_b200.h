@@ -468,8 +468,8 @@ int hb_debug_rowwise_compile(const hb_rowwise_args* args, char* source, int64_t 
  * page table behind a sequence's last page are not read.  What the device finds wrong in them it leaves out and reports
  * through hb_cache_status: a page outside of [0, num_pages) (its tokens are not written, and are not seen by any query), a
  * length beyond max_pages * page_size (attention takes it as that, append leaves out the tokens behind it), more rows than the sequence
- * is long, a position behind the rotary tables (neither written), starts that leave [0, T] (taken as the nearest that do not).  Where starts then descend, rows would belong to two
- * sequences: such a call writes nothing at all, and is reported.
+ * is long, a position behind the rotary tables (neither written), starts that leave [0, T] (taken as the nearest that do not).  Where
+ * starts then descend, rows would belong to two sequences: such a call writes nothing at all, and is reported.
  * A page whose key scale is 0 in a head holds nothing there yet, as every page before its first append: it is not seen either, and that
  * is not reported.  A value scale of 0 makes the page's values 0.
  * page_size 16, 32, 64 or 128; D 64 or 128.

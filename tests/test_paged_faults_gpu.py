@@ -127,7 +127,7 @@ def test_reports_are_not_lost_while_others_are_read(built_lib):
                     for bits in reads[max(before - 1, 0):]:  # the last one may have begun before
                         got |= bits
                 assert got == 3, (n, got)
-                while len(reads) < before + 4 and time.monotonic() < until and not failed:  # nothing of this round is left for the next one
+                while len(reads) < before + 4 and time.monotonic() < until and not failed:  # nothing is left for the next pass
                     pass
     finally:
         stop.set()
